@@ -750,6 +750,53 @@ int nnz_layer_norm_backward_partial(const float* x, const float* gamma, const fl
                                     const float* dres, float* dx, float* part, long rows, int C, int pad_h, int pad_w,
                                     int pad_y, int pad_x, void* stream);
 
+/* ---- group norm with an activation, channels last (monai get_norm_layer(("GROUP", ..)) + get_act_layer in the residual blocks,
+ * nets/lm2net.py:119-121,160-171, light_mamba2net.py:480-482,519-531, LightMUNet.py:105-107,144-156).  x: [N][S][C], batch and row
+ * strides in elements, C innermost; y, dy, dx contiguous.  Element types 0: fp32, 1: fp16, 2: bf16; y / dy have x's type or fp32.
+ * act 0: none, 1: ReLU, 2: LeakyReLU(slope), 3: SiLU.  stats: [N][G][2] = mean, 1 / sqrt(var + eps), written by the forward and read
+ * by the backward.  weight / bias fp32 [C] or NULL; dweight / dbias [C] or NULL.  C <= 4096.  Bit-identical from run to run. */
+long nnz_group_norm_act_workspace_bytes(long N, long S, int C, int G, int backward);
+int nnz_group_norm_act_forward(const void* x, int x_type, long x_batch_stride, long x_row_stride, const float* weight,
+                               const float* bias, void* y, int y_type, float* stats, void* workspace, long workspace_bytes,
+                               long N, long S, int C, int G, float eps, int act, float slope, void* stream);
+int nnz_group_norm_act_backward(const void* x, int x_type, long x_batch_stride, long x_row_stride, const void* dy, int dy_type,
+                                const float* weight, const float* bias, const float* stats, void* dx, float* dweight,
+                                float* dbias, void* workspace, long workspace_bytes, long N, long S, int C, int G, int act,
+                                float slope, void* stream);
+
+/* ---- dropout from a counter-based generator, beside the residual + DropPath operator (nn.Dropout of nets/m2net.py:70,166,
+ * mamba_nd2net.py:118, swt2net.py:181-183): element e is kept iff its 32-bit draw >= threshold (0 .. 2^32), y = kept ? x * scale : 0
+ * [+ residual].  Draws: csrc/dropout.hip.  state / used: device {seed, step}; the forward copies the pair it read to `used` (may be
+ * NULL) for its backward.  y has the wider of the types of x and residual (fp16 beside bf16: fp32). */
+int nnz_dropout_forward(const void* x, int x_type, const void* residual, int residual_type, void* y, long n, long threshold,
+                        float scale, int site, const long long* state, long long* used, void* stream);
+int nnz_dropout_backward(const void* dy, int dy_type, void* dx, int dx_type, long n, long threshold, float scale, int site,
+                         const long long* used, void* stream);
+
+/* ---- the state-carrying operators of the 1-D Mamba blocks, token-major (Mamba.step and inference_params,
+ * nets/seg_mamba/mamba_simple.py:190-215, 357-411).  type: element type of the activations.  conv_state [B][D][W] (any strides,
+ * element type state_type; NULL in the prompt form: zeros, nothing kept) and state [B][D][N] fp32 (contiguous within a sequence)
+ * are updated in place.  lengths: [B] int32 / int64 device or NULL; active: [B] bytes or NULL.  W <= 8; N 4, 8, 16, 32.
+ * strides (host table, elements): prompt {x batch, x token, dt batch, dt token, B batch, B token, B group, C batch, C token,
+ * C group, z batch, z token}; token {x batch, dt batch, B batch, B group, C batch, C group, z batch}. */
+int nnz_causal_conv1d_prompt(const void* x, int type, long x_batch_stride, long x_token_stride, const float* weight,
+                             const float* bias, void* y, void* conv_state, int state_type, long state_batch_stride,
+                             long state_channel_stride, long state_column_stride, const void* lengths, int lengths_are_int64,
+                             int B, int L, int D, int W, int silu, void* stream);
+int nnz_causal_conv1d_token(const void* x, int type, long x_batch_stride, const float* weight, const float* bias, void* y,
+                            void* conv_state, int state_type, long state_batch_stride, long state_channel_stride,
+                            long state_column_stride, const void* active, int B, int D, int W, int silu, void* stream);
+long nnz_selective_scan_prompt_workspace_bytes(int B, int L, int D, int H, int G, int N);
+int nnz_selective_scan_prompt(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
+                              const long* strides, const float* A, int A_per_state, const float* D_skip, const float* dt_bias,
+                              int softplus, float* state, long state_batch_stride, void* y, const void* lengths,
+                              int lengths_are_int64, void* workspace, long workspace_bytes, int B, int L, int D, int H, int G,
+                              int N, void* stream);
+int nnz_selective_scan_token(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
+                             const long* strides, const float* A, int A_per_state, const float* D_skip, const float* dt_bias,
+                             int softplus, float* state, long state_batch_stride, void* y, const void* active, int B, int D,
+                             int H, int G, int N, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

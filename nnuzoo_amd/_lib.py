@@ -247,6 +247,17 @@ SIGNATURES = {
     "nnz_selective_scan_grad_state_floats": [_i, _i, _i],
     "nnz_selective_scan_forward": [_fp] * 10 + [_i] * 6 + [_vp],
     "nnz_selective_scan_backward": [_fp] * 18 + [_i] * 6 + [_vp],
+    "nnz_group_norm_act_workspace_bytes": [_l, _l, _i, _i, _i],
+    "nnz_group_norm_act_forward": [_vp, _i, _l, _l, _fp, _fp, _vp, _i, _fp, _vp, _l, _l, _l, _i, _i, _f, _i, _f, _vp],
+    "nnz_group_norm_act_backward": [_vp, _i, _l, _l, _vp, _i, _fp, _fp, _fp, _vp, _fp, _fp, _vp, _l, _l, _l, _i, _i, _i, _f, _vp],
+    "nnz_dropout_forward": [_vp, _i, _vp, _i, _vp, _l, _l, _f, _i, _vp, _vp, _vp],
+    "nnz_dropout_backward": [_vp, _i, _vp, _i, _l, _l, _f, _i, _vp, _vp],
+    "nnz_causal_conv1d_prompt": [_vp, _i, _l, _l, _fp, _fp, _vp, _vp, _i, _l, _l, _l, _vp, _i, _i, _i, _i, _i, _i, _vp],
+    "nnz_causal_conv1d_token": [_vp, _i, _l, _fp, _fp, _vp, _vp, _i, _l, _l, _l, _vp, _i, _i, _i, _i, _vp],
+    "nnz_selective_scan_prompt_workspace_bytes": [_i] * 6,
+    "nnz_selective_scan_prompt": [_vp] * 5 + [_i, C.POINTER(C.c_long), _fp, _i, _fp, _fp, _i, _fp, _l, _vp, _vp, _i, _vp, _l]
+                                 + [_i] * 6 + [_vp],
+    "nnz_selective_scan_token": [_vp] * 5 + [_i, C.POINTER(C.c_long), _fp, _i, _fp, _fp, _i, _fp, _l, _vp, _vp] + [_i] * 5 + [_vp],
 }
 
 _LONG_RESULT = {"nnz_aug_stats_workspace_floats", "nnz_ss2d_scan_state_floats", "nnz_ss2d_scan_grad_state_floats", "nnz_ss2d_scan_workspace_floats",
@@ -257,7 +268,8 @@ _LONG_RESULT = {"nnz_aug_stats_workspace_floats", "nnz_ss2d_scan_state_floats", 
                 "nnz_window_attention_backward_parts",
                 "nnz_ss2d_xproj_backward_w_workspace_floats", "nnz_ss2d_dwconv_silu_backward_workspace_floats",
                 "nnz_dw3x3_nhwc_wgrad_workspace_floats", "nnz_pw_wgrad_small_workspace_floats",
-                "nnz_head1x1_wgrad_workspace_floats", "nnz_pw_wgrad_small_workspace_floats_b"}
+                "nnz_head1x1_wgrad_workspace_floats", "nnz_pw_wgrad_small_workspace_floats_b",
+                "nnz_group_norm_act_workspace_bytes", "nnz_selective_scan_prompt_workspace_bytes"}
 _lib = None
 
 

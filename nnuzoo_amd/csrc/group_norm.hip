@@ -1,0 +1,472 @@
+// Group norm with an activation, channels last (gfx950), forward and backward:
+//   z = (x - mu[n,g]) * r[n,g] * w[c] + b[c],  y = act(z),  mu / r over the S positions and C / G channels of a group;
+//   dz = dy act'(z),  db = sum dz,  dw = sum dz xhat,  dx = r (w dz - <w dz> - xhat <w dz xhat>)  with <.> the group's mean.
+// Bound by HBM: a group does not fit on chip, so forward reads x twice and writes y, backward reads x and dy twice and writes dx.
+//
+// A thread owns V consecutive channels (16 bytes) and walks the rows, a workgroup owns a run of rows of one sample: every access
+// is a run of whole rows whatever the group width, and the group's members meet only after the rows are summed.  Sums of the
+// forward are kept in fp64 (the vector rate of fp64 FMA is that of plain fp32 here, and E[x^2] - mu^2 then loses nothing
+// that fp32 statistics could hold, whatever mu / sigma is); partial sums go to a workspace and are added in a fixed order, so
+// results are bit-identical from run to run.  No atomics.
+#include "elem_io.hpp"
+
+namespace nnz {
+
+enum GnAct { GN_NONE = 0, GN_RELU = 1, GN_LEAKY = 2, GN_SILU = 3 };
+constexpr int GN_NT = 256;
+
+struct GnArgs {
+  const void* x;      // [N][S][C] with strides xb, xs, 1
+  const void* dy;     // [N][S][C] contiguous
+  const float* w;     // [C] or null (ones)
+  const float* b;     // [C] or null (zeros)
+  void* out;          // y or dx, [N][S][C] contiguous
+  float* stats;       // [N][G][2]: mean, 1 / sqrt(var + eps)
+  double* gpart;      // [N][nblk][G][2]
+  float* cpart;       // backward: [N][nblk][C][2]: sum dz, sum dz xhat
+  float* cc;          // backward: [N][G][2]: <w dz>, <w dz xhat>
+  float* dw;          // [C] or null
+  float* db;
+  long N, S, xb, xs, rows;  // rows: of one workgroup
+  int nblk, C, G, q;        // q = C / G
+  int act;
+  float slope, eps;
+};
+
+__device__ __forceinline__ float gn_act(float z, int act, float slope) {
+  switch (act) {
+    case GN_RELU: return z < 0.f ? 0.f : z;  // NaN stays
+    case GN_LEAKY: return z > 0.f ? z : z * slope;
+    case GN_SILU: return z * sigmoid_hw(z);
+    default: return z;
+  }
+}
+__device__ __forceinline__ float gn_dact(float z, float dy, int act, float slope) {
+  switch (act) {
+    case GN_RELU: return z > 0.f ? dy : 0.f;
+    case GN_LEAKY: return z > 0.f ? dy : dy * slope;
+    case GN_SILU: {
+      const float s = sigmoid_hw(z);
+      return dy * (s * (1.f + z * (1.f - s)));
+    }
+    default: return dy;
+  }
+}
+
+// a thread's place: vector columns [c0, c0 + cw) of the row are dealt out over the workgroup, R rows at a time
+struct GnPlace {
+  int col, rr, R;
+  bool on;
+};
+__device__ __forceinline__ GnPlace gn_place(int cw) {
+  GnPlace p;
+  p.R = GN_NT / cw;
+  p.rr = threadIdx.x / cw;
+  p.col = threadIdx.x - p.rr * cw;
+  p.on = p.rr < p.R;
+  return p;
+}
+
+// per-channel sums over the workgroup's row threads: v[V] of every thread -> dst[channel], in a fixed order
+template <class A, int V>
+__device__ __forceinline__ void gn_fold_rows(A* stage, A* dst, const A (&v)[V], const GnPlace& p, int cw) {
+  __syncthreads();
+  if (p.on) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) stage[threadIdx.x * V + j] = v[j];
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < cw * V; c += GN_NT) {
+    A s = 0;
+    for (int r = 0; r < p.R; ++r) s += stage[r * cw * V + c];
+    dst[c] = s;
+  }
+}
+
+template <class TI, int V>
+__global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) double gn_lds_d[];
+  double* stage = gn_lds_d;             // [GN_NT * V]
+  double* sums = gn_lds_d + GN_NT * V;  // [2][C]
+  const long n = blockIdx.x / a.nblk;
+  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
+  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const TI* xn = (const TI*)a.x + n * a.xb;
+  const int CV = a.C / V;
+  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+    const GnPlace p = gn_place(cw);
+    double s[V], sq[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = sq[j] = 0.0;
+    if (p.on) {
+      const TI* xc = xn + (long)(c0 + p.col) * V;
+#pragma unroll 4
+      for (long r = r0 + p.rr; r < r1; r += p.R) {
+        float v[V];
+        ld_elems<TI, V>(xc + r * a.xs, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double d = (double)v[j];
+          s[j] += d;
+          sq[j] = fma(d, d, sq[j]);
+        }
+      }
+    }
+    gn_fold_rows<double, V>(stage, sums + c0 * V, s, p, cw);
+    gn_fold_rows<double, V>(stage, sums + a.C + c0 * V, sq, p, cw);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < a.G; g += GN_NT) {
+    double s = 0.0, sq = 0.0;
+    for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
+      s += sums[c];
+      sq += sums[a.C + c];
+    }
+    double* o = a.gpart + ((long)blockIdx.x * a.G + g) * 2;
+    o[0] = s;
+    o[1] = sq;
+  }
+}
+
+// pairs [nblk] of one (sample, group) summed by one wave
+__device__ __forceinline__ void gn_sum_parts(const double* p, int nblk, int G, double& s, double& t) {
+  s = t = 0.0;
+  for (int k = threadIdx.x & 63; k < nblk; k += 64) {
+    s += p[(long)k * G * 2];
+    t += p[(long)k * G * 2 + 1];
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    t += __shfl_xor(t, o, 64);
+  }
+}
+
+__global__ __launch_bounds__(64) void gn_stats_finish_kernel(GnArgs a) {
+  const long n = blockIdx.x / a.G;
+  const int g = (int)(blockIdx.x - n * a.G);
+  double s, sq;
+  gn_sum_parts(a.gpart + (n * a.nblk * a.G + g) * 2, a.nblk, a.G, s, sq);
+  if (threadIdx.x == 0) {
+    const double m = (double)a.S * a.q, mean = s / m;
+    double var = sq / m - mean * mean;
+    if (var < 0.0) var = 0.0;  // NaN stays
+    a.stats[(long)blockIdx.x * 2] = (float)mean;
+    a.stats[(long)blockIdx.x * 2 + 1] = (float)(1.0 / sqrt(var + (double)a.eps));
+  }
+}
+
+// per-channel constants of a thread's V channels
+template <int V>
+struct GnChan {
+  float mean[V], rstd[V], w[V], b[V];
+};
+template <int V>
+__device__ __forceinline__ void gn_chan(const GnArgs& a, long n, int c, GnChan<V>& k) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float* st = a.stats + (n * a.G + (c + j) / a.q) * 2;
+    k.mean[j] = st[0];
+    k.rstd[j] = st[1];
+    k.w[j] = a.w ? a.w[c + j] : 1.f;
+    k.b[j] = a.b ? a.b[c + j] : 0.f;
+  }
+}
+
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(GN_NT) void gn_apply_kernel(GnArgs a) {
+  const long n = blockIdx.x / a.nblk;
+  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
+  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const TI* xn = (const TI*)a.x + n * a.xb;
+  TO* yn = (TO*)a.out + n * a.S * a.C;
+  const int CV = a.C / V;
+  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+    const GnPlace p = gn_place(cw);
+    if (!p.on) continue;
+    const int c = (c0 + p.col) * V;
+    GnChan<V> k;
+    gn_chan<V>(a, n, c, k);
+#pragma unroll 2
+    for (long r = r0 + p.rr; r < r1; r += p.R) {
+      float v[V];
+      ld_elems<TI, V>(xn + r * a.xs + c, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = gn_act(fmaf((v[j] - k.mean[j]) * k.rstd[j], k.w[j], k.b[j]), a.act, a.slope);
+      st_elems<TO, V>(yn + r * a.C + c, v);
+    }
+  }
+}
+
+// backward sums: per channel sum dz and sum dz xhat of the workgroup's rows, and their weighted sums per group
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(GN_NT) void gn_bwd_reduce_kernel(GnArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float gn_lds_f[];
+  float* stage = gn_lds_f;             // [GN_NT * V]
+  float* sums = gn_lds_f + GN_NT * V;  // [2][C]
+  const long n = blockIdx.x / a.nblk;
+  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
+  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const TI* xn = (const TI*)a.x + n * a.xb;
+  const TO* gn = (const TO*)a.dy + n * a.S * a.C;
+  const int CV = a.C / V;
+  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+    const GnPlace p = gn_place(cw);
+    float s[V], t[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = t[j] = 0.f;
+    if (p.on) {
+      const int c = (c0 + p.col) * V;
+      GnChan<V> k;
+      gn_chan<V>(a, n, c, k);
+#pragma unroll 2
+      for (long r = r0 + p.rr; r < r1; r += p.R) {
+        float v[V], g[V];
+        ld_elems<TI, V>(xn + r * a.xs + c, v);
+        ld_elems<TO, V>(gn + r * a.C + c, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = (v[j] - k.mean[j]) * k.rstd[j];
+          const float dz = gn_dact(fmaf(xh, k.w[j], k.b[j]), g[j], a.act, a.slope);
+          s[j] += dz;
+          t[j] = fmaf(dz, xh, t[j]);
+        }
+      }
+    }
+    gn_fold_rows<float, V>(stage, sums + c0 * V, s, p, cw);
+    gn_fold_rows<float, V>(stage, sums + a.C + c0 * V, t, p, cw);
+  }
+  __syncthreads();
+  float* cp = a.cpart + (long)blockIdx.x * a.C * 2;
+  for (int c = threadIdx.x; c < a.C; c += GN_NT) {
+    cp[2 * c] = sums[c];
+    cp[2 * c + 1] = sums[a.C + c];
+  }
+  for (int g = threadIdx.x; g < a.G; g += GN_NT) {
+    double s = 0.0, t = 0.0;
+    for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
+      const double w = a.w ? a.w[c] : 1.0;
+      s += w * sums[c];
+      t += w * sums[a.C + c];
+    }
+    double* o = a.gpart + ((long)blockIdx.x * a.G + g) * 2;
+    o[0] = s;
+    o[1] = t;
+  }
+}
+
+constexpr int GN_FC = 4;  // channels of a finishing workgroup: 4 x 64 threads share the partial sums of 4 channels
+// workgroups 0 .. N * G / 4 (rounded up): <w dz>, <w dz xhat> of 4 (sample, group) pairs, a wave each; the rest: dw and db
+__global__ __launch_bounds__(GN_NT) void gn_bwd_finish_kernel(GnArgs a, long pair_wgs) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if ((long)blockIdx.x < pair_wgs) {
+    const long pair = (long)blockIdx.x * 4 + wave;
+    if (pair >= a.N * a.G) return;
+    const long n = pair / a.G;
+    double s, t;
+    gn_sum_parts(a.gpart + (n * a.nblk * a.G + (pair - n * a.G)) * 2, a.nblk, a.G, s, t);
+    if (lane == 0) {
+      const double m = (double)a.S * a.q;
+      a.cc[pair * 2] = (float)(s / m);
+      a.cc[pair * 2 + 1] = (float)(t / m);
+    }
+    return;
+  }
+  // lanes 4k + i of the workgroup's 256: partial k, k + 64, .. of channel i
+  const int c = (int)((long)blockIdx.x - pair_wgs) * GN_FC + (threadIdx.x & (GN_FC - 1));
+  const long parts = a.N * a.nblk;
+  double s = 0.0, t = 0.0;
+  if (c < a.C) {
+    const float* cp = a.cpart + 2 * (long)c;
+#pragma unroll 8
+    for (long k = threadIdx.x / GN_FC; k < parts; k += GN_NT / GN_FC) {
+      s += cp[k * a.C * 2];
+      t += cp[k * a.C * 2 + 1];
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= GN_FC; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    t += __shfl_xor(t, o, 64);
+  }
+  __shared__ double red[4][GN_FC][2];
+  if (lane < GN_FC) {
+    red[wave][lane][0] = s;
+    red[wave][lane][1] = t;
+  }
+  __syncthreads();
+  if (threadIdx.x < GN_FC && c < a.C) {
+    if (a.db) a.db[c] = (float)((red[0][lane][0] + red[1][lane][0]) + (red[2][lane][0] + red[3][lane][0]));
+    if (a.dw) a.dw[c] = (float)((red[0][lane][1] + red[1][lane][1]) + (red[2][lane][1] + red[3][lane][1]));
+  }
+}
+
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
+  const long n = blockIdx.x / a.nblk;
+  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
+  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const TI* xn = (const TI*)a.x + n * a.xb;
+  const TO* gn = (const TO*)a.dy + n * a.S * a.C;
+  TI* on = (TI*)a.out + n * a.S * a.C;
+  const int CV = a.C / V;
+  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+    const GnPlace p = gn_place(cw);
+    if (!p.on) continue;
+    const int c = (c0 + p.col) * V;
+    GnChan<V> k;
+    gn_chan<V>(a, n, c, k);
+    float m1[V], m2[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float* cc = a.cc + (n * a.G + (c + j) / a.q) * 2;
+      m1[j] = cc[0];
+      m2[j] = cc[1];
+    }
+#pragma unroll 2
+    for (long r = r0 + p.rr; r < r1; r += p.R) {
+      float v[V], g[V];
+      ld_elems<TI, V>(xn + r * a.xs + c, v);
+      ld_elems<TO, V>(gn + r * a.C + c, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xh = (v[j] - k.mean[j]) * k.rstd[j];
+        const float dz = gn_dact(fmaf(xh, k.w[j], k.b[j]), g[j], a.act, a.slope);
+        v[j] = k.rstd[j] * (k.w[j] * dz - m1[j] - xh * m2[j]);
+      }
+      st_elems<TI, V>(on + r * a.C + c, v);
+    }
+  }
+}
+
+constexpr int GN_MAX_C = 4096;    // 2 x C fp64 sums and 256 x V fp64 staging fit LDS
+constexpr long GN_TARGET = 1024;  // workgroups of a launch
+// rows of a workgroup: enough workgroups to fill the chip, at least 8 passes over the rows that its threads cover at once
+inline void gn_split(GnArgs& a, int V) {
+  const int CV = a.C / V;
+  const long R = CV >= GN_NT ? 1 : GN_NT / CV;
+  long per = (GN_TARGET + a.N - 1) / a.N;
+  const long most = (a.S + 8 * R - 1) / (8 * R);
+  if (per > most) per = most;
+  if (per < 1) per = 1;
+  a.rows = (a.S + per - 1) / per;
+  a.nblk = (int)((a.S + a.rows - 1) / a.rows);
+}
+inline long gn_align(long v) { return (v + 255) & ~255L; }
+// layout of the workspace, the same whatever V a call's alignment allows
+struct GnWs {
+  long gpart, cpart, cc, bytes;
+};
+inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
+  long parts = (GN_TARGET + N - 1) / N;   // no split has more parts a sample
+  if (parts > S) parts = S;
+  GnWs w;
+  w.gpart = 0;
+  w.cpart = gn_align(N * parts * G * 16);
+  w.cc = w.cpart + (bwd ? gn_align(N * parts * C * 8) : 0);
+  w.bytes = w.cc + (bwd ? gn_align(N * G * 8) : 0);
+  return w;
+}
+
+template <class TI, class TO, int V>
+static int gn_run_fwd(GnArgs a, hipStream_t s) {
+  static DynLdsCache cache;
+  gn_split(a, V);
+  const int lds = (GN_NT * V + 2 * a.C) * 8;
+  hipError_t e = ensure_dyn_lds((const void*)gn_stats_kernel<TI, V>, lds, cache);
+  if (e != hipSuccess) return (int)e;
+  const dim3 grid((unsigned)(a.N * a.nblk));
+  NNZ_LAUNCH((gn_stats_kernel<TI, V>), grid, dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH_CHECK();
+  NNZ_LAUNCH(gn_stats_finish_kernel, dim3((unsigned)(a.N * a.G)), dim3(64), 0, s, a);
+  NNZ_LAUNCH_CHECK();
+  NNZ_LAUNCH((gn_apply_kernel<TI, TO, V>), grid, dim3(GN_NT), 0, s, a);
+  NNZ_LAUNCH_CHECK();
+  return NNZ_OK;
+}
+template <class TI, class TO, int V>
+static int gn_run_bwd(GnArgs a, hipStream_t s) {
+  static DynLdsCache cache;
+  gn_split(a, V);
+  const int lds = (GN_NT * V + 2 * a.C) * 4;
+  hipError_t e = ensure_dyn_lds((const void*)gn_bwd_reduce_kernel<TI, TO, V>, lds, cache);
+  if (e != hipSuccess) return (int)e;
+  const dim3 grid((unsigned)(a.N * a.nblk));
+  NNZ_LAUNCH((gn_bwd_reduce_kernel<TI, TO, V>), grid, dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH_CHECK();
+  const long pair_wgs = (a.N * a.G + 3) / 4;
+  NNZ_LAUNCH(gn_bwd_finish_kernel, dim3((unsigned)(pair_wgs + (a.C + GN_FC - 1) / GN_FC)), dim3(GN_NT), 0, s, a, pair_wgs);
+  NNZ_LAUNCH_CHECK();
+  NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V>), grid, dim3(GN_NT), 0, s, a);
+  NNZ_LAUNCH_CHECK();
+  return NNZ_OK;
+}
+
+// V: the widest of 16 bytes, 4 elements and 1 that the channel count, the strides and the pointers allow
+template <class TI, class TO>
+static int gn_dispatch(const GnArgs& a, bool bwd, hipStream_t s) {
+  auto fits = [&](int v) {
+    const uintptr_t ai = (v * sizeof(TI) < 16 ? v * sizeof(TI) : 16) - 1, ao = (v * sizeof(TO) < 16 ? v * sizeof(TO) : 16) - 1;
+    const uintptr_t out = (uintptr_t)a.out & (bwd ? ai : ao), dy = bwd ? ((uintptr_t)a.dy & ao) : 0;
+    return a.C % v == 0 && a.xs % v == 0 && a.xb % v == 0 && ((uintptr_t)a.x & ai) == 0 && out == 0 && dy == 0;
+  };
+  constexpr int FULL = 16 / (int)sizeof(TI);
+  if (fits(FULL)) return bwd ? gn_run_bwd<TI, TO, FULL>(a, s) : gn_run_fwd<TI, TO, FULL>(a, s);
+  if (FULL != 4 && fits(4)) return bwd ? gn_run_bwd<TI, TO, 4>(a, s) : gn_run_fwd<TI, TO, 4>(a, s);
+  return bwd ? gn_run_bwd<TI, TO, 1>(a, s) : gn_run_fwd<TI, TO, 1>(a, s);
+}
+static int gn_go(const GnArgs& a, int ti, int to, bool bwd, hipStream_t s) {
+  if (ti == ELEM_F32 && to == ELEM_F32) return gn_dispatch<float, float>(a, bwd, s);
+  if (ti == ELEM_F16 && to == ELEM_F16) return gn_dispatch<f16, f16>(a, bwd, s);
+  if (ti == ELEM_F16 && to == ELEM_F32) return gn_dispatch<f16, float>(a, bwd, s);
+  if (ti == ELEM_BF16 && to == ELEM_BF16) return gn_dispatch<bf16, bf16>(a, bwd, s);
+  if (ti == ELEM_BF16 && to == ELEM_F32) return gn_dispatch<bf16, float>(a, bwd, s);
+  return NNZ_EINVAL;
+}
+static bool gn_shape_ok(long N, long S, int C, int G) {
+  return N >= 1 && S >= 1 && C >= 1 && C <= GN_MAX_C && G >= 1 && C % G == 0 && N <= (1L << 28) / G && S <= (1L << 40) / C / N;
+}
+
+}  // namespace nnz
+
+extern "C" long nnz_group_norm_act_workspace_bytes(long N, long S, int C, int G, int backward) {
+  using namespace nnz;
+  if (!gn_shape_ok(N, S, C, G)) return NNZ_EINVAL;
+  return gn_ws(N, S, C, G, backward != 0).bytes;
+}
+
+extern "C" int nnz_group_norm_act_forward(const void* x, int x_type, long x_batch_stride, long x_row_stride, const float* weight,
+                                          const float* bias, void* y, int y_type, float* stats, void* workspace,
+                                          long workspace_bytes, long N, long S, int C, int G, float eps, int act, float slope,
+                                          void* stream) {
+  using namespace nnz;
+  if (!x || !y || !stats || !workspace || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
+  const GnWs w = gn_ws(N, S, C, G, false);
+  if (workspace_bytes < w.bytes) return NNZ_EINVAL;
+  GnArgs a = {};
+  a.x = x; a.w = weight; a.b = bias; a.out = y; a.stats = stats; a.gpart = (double*)workspace;
+  a.N = N; a.S = S; a.xb = x_batch_stride; a.xs = x_row_stride; a.C = C; a.G = G; a.q = C / G;
+  a.act = act; a.slope = slope; a.eps = eps;
+  return gn_go(a, x_type, y_type, false, (hipStream_t)stream);
+}
+
+extern "C" int nnz_group_norm_act_backward(const void* x, int x_type, long x_batch_stride, long x_row_stride, const void* dy,
+                                           int dy_type, const float* weight, const float* bias, const float* stats, void* dx,
+                                           float* dweight, float* dbias, void* workspace, long workspace_bytes, long N, long S,
+                                           int C, int G, int act, float slope, void* stream) {
+  using namespace nnz;
+  if (!x || !dy || !dx || !stats || !workspace || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
+  const GnWs w = gn_ws(N, S, C, G, true);
+  if (workspace_bytes < w.bytes) return NNZ_EINVAL;
+  GnArgs a = {};
+  a.x = x; a.dy = dy; a.w = weight; a.b = bias; a.out = dx; a.stats = (float*)stats;
+  a.gpart = (double*)workspace; a.cpart = (float*)((char*)workspace + w.cpart); a.cc = (float*)((char*)workspace + w.cc);
+  a.dw = dweight; a.db = dbias;
+  a.N = N; a.S = S; a.xb = x_batch_stride; a.xs = x_row_stride; a.C = C; a.G = G; a.q = C / G;
+  a.act = act; a.slope = slope;
+  return gn_go(a, x_type, dy_type, true, (hipStream_t)stream);
+}

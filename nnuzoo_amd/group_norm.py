@@ -1,0 +1,158 @@
+"""Group norm with an activation on channels-last tensors, on the kernels of csrc/group_norm.hip: what nn.GroupNorm followed by
+an activation computes in the residual blocks of the LightMUNet family (reference: monai's get_norm_layer / get_act_layer at
+nnunetv2/nets/lm2net.py:119-121,160-171, light_mamba2net.py:480-482,519-531, LightMUNet.py:105-107,144-156), one operator with its
+gradient.
+
+  group_norm_act(x, num_groups, weight, bias, eps, activation, negative_slope)      x (N, *spatial, C), C innermost
+  GroupNormAct(num_groups, num_channels, ..., activation=...)                       nn.GroupNorm's parameters, x (N, C, *spatial)
+  norm_act(norm, act, x)                                                            act(norm(x)) of two modules on either path
+
+fp32 / fp16 / bf16 in; the output has the input's type, or fp32 under autocast (group_norm is on autocast's fp32 list).
+Statistics are fp64 sums, everything else is computed in fp32 and rounded once.  Results are bit-identical from run to run."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from ._lib import load, ptr
+from .launch import ELEM, launch, need_device, need_elem
+
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
+MAX_CHANNELS = 4096     # csrc/group_norm.hip GN_MAX_C
+
+
+def _rows(x: torch.Tensor):
+    """(x or its contiguous copy, batch stride, row stride): rows of C adjacent elements, evenly spaced within a sample"""
+    C = x.shape[-1]
+    if x.stride(-1) == 1 or C == 1:
+        step = x.stride(-2) if x.dim() > 2 else C
+        want = step
+        for d in range(x.dim() - 2, 0, -1):
+            if x.shape[d] != 1 and x.stride(d) != want:
+                break
+            want *= x.shape[d]
+        else:
+            return x, x.stride(0), step
+    x = x.contiguous()
+    return x, x.numel() // max(1, x.shape[0]), C
+
+
+class _GroupNormActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, slope, out_dtype):
+        dev = x.device
+        x, xb, xs = _rows(x)
+        N, C = x.shape[0], x.shape[-1]
+        y = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        ctx.cfg = (xb, xs, groups, act, slope)
+        ctx.affine = (weight is not None, bias is not None)
+        if y.numel() == 0:
+            ctx.save_for_backward(x, weight, bias, None)
+            return y
+        S = x.numel() // (N * C)
+        ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 0)
+        ws = torch.empty(max(ws_bytes, 0), dtype=torch.uint8, device=dev)
+        stats = torch.empty(2 * N * groups, dtype=torch.float32, device=dev)
+        launch("nnz_group_norm_act_forward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, ptr(weight), ptr(bias), y.data_ptr(),
+               ELEM[out_dtype], stats.data_ptr(), ws.data_ptr(), ws_bytes, N, S, C, groups, eps, act, slope)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        xb, xs, groups, act, slope = ctx.cfg
+        dev, N, C = x.device, x.shape[0], x.shape[-1]
+        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+        make = torch.empty if stats is not None else torch.zeros
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        affine = make((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
+        dw, db = (affine[0] if need_w else None), (affine[1] if need_b else None)
+        if stats is not None:
+            dy = dy.contiguous()
+            S = x.numel() // (N * C)
+            ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
+            ws = torch.empty(max(ws_bytes, 0), dtype=torch.uint8, device=dev)
+            launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
+                   ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ws.data_ptr(), ws_bytes, N, S, C,
+                   groups, act, slope)
+        return dx, dw, db, None, None, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-5, activation: Optional[str] = None,
+                   negative_slope: float = 0.01) -> torch.Tensor:
+    """activation(group_norm(x)) for x (N, *spatial, C); activation: None / "none", "relu", "leaky_relu", "silu"."""
+    dev = need_device("group_norm_act", x, weight, bias)
+    need_elem("group_norm_act", x=x, weight=weight, bias=bias)
+    if activation not in ACTIVATIONS:
+        raise NotImplementedError(f"group_norm_act: activation {activation!r} (one of {sorted(k for k in ACTIVATIONS if k)})")
+    if x.dim() < 2:
+        raise ValueError(f"group_norm_act: x must be (N, *spatial, C), got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C % num_groups or C < 1:
+        raise ValueError(f"group_norm_act: {C} channels in {num_groups} groups")
+    if C > MAX_CHANNELS:
+        raise NotImplementedError(f"group_norm_act: at most {MAX_CHANNELS} channels, got {C}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and tuple(p.shape) != (C,):
+            raise ValueError(f"group_norm_act: `{name}` has shape {tuple(p.shape)}, expected ({C},)")
+    weight, bias = (p if p is None else p.float().contiguous() for p in (weight, bias))
+    out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
+    return _GroupNormActFn.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation], float(negative_slope),
+                                 out_dtype)
+
+
+class GroupNormAct(nn.GroupNorm):
+    """nn.GroupNorm (same constructor, parameters, state_dict) followed by an activation, for x (N, C, *spatial): a tensor whose
+    channels lie innermost (torch.channels_last, token-major views) is read in place and the output has the same layout; any
+    other layout is copied to it first."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, device=None, dtype=None,
+                 activation: Optional[str] = None, negative_slope: float = 0.01):
+        super().__init__(num_groups, num_channels, eps, affine, device=device, dtype=dtype)
+        if activation not in ACTIVATIONS:
+            raise NotImplementedError(f"GroupNormAct: activation {activation!r}")
+        self.activation, self.negative_slope = activation, negative_slope
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = group_norm_act(x.movedim(1, -1), self.num_groups, self.weight, self.bias, self.eps, self.activation,
+                           self.negative_slope)
+        return y.movedim(-1, 1)
+
+    def extra_repr(self) -> str:
+        return f"{super().extra_repr()}, activation={self.activation}"
+
+
+def _token_order(x: torch.Tensor):
+    """the permutation that turns x (N, C, *spatial) into contiguous (N, *spatial in memory order, C), or None where there is none
+    or where x is just as well stored channel by channel"""
+    if x.dim() < 3 or x.shape[1] < 2 or x.is_contiguous():
+        return None
+    perm = (0, *sorted(range(2, x.dim()), key=lambda d: -x.stride(d)), 1)
+    return perm if x.permute(perm).is_contiguous() else None
+
+
+def _hooked(m: nn.Module) -> bool:
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def norm_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
+    """act(norm(x)): the operator where `norm` is an nn.GroupNorm, `act` one of its activations and x a device tensor whose channels
+    lie innermost (what the token-major mixers of the LightMUNet family hand on; the spatial axes may lie in any order); the two
+    modules one after the other otherwise."""
+    name = {nn.ReLU: "relu", nn.SiLU: "silu", nn.LeakyReLU: "leaky_relu", nn.Identity: "none"}.get(type(act))
+    if (type(norm) is nn.GroupNorm and name is not None and x.is_cuda and x.dtype in ELEM and norm.num_channels <= MAX_CHANNELS
+            and not _hooked(norm) and not _hooked(act)):
+        perm = _token_order(x)
+        if perm is not None:
+            from . import backends
+            backends.note(norm, "hip", "group norm + activation")
+            y = group_norm_act(x.permute(perm), norm.num_groups, norm.weight, norm.bias, norm.eps, name,
+                               getattr(act, "negative_slope", 0.01))
+            return y.permute([perm.index(d) for d in range(x.dim())])
+    return act(norm(x))

@@ -1,0 +1,40 @@
+"""What the operators with fp32 / fp16 / bf16 tensors share on the host: element types as the C boundary names them, and a launch
+on the tensors' own device and that device's current stream."""
+from __future__ import annotations
+
+import torch
+
+from ._lib import HipCallError, check, load
+
+ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def need_device(name: str, *tensors) -> torch.device:
+    """the one device of all tensors (None is skipped); CPU tensors and mixed devices are refused"""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"nnuzoo_amd.{name} runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise HipCallError(f"{name}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def need_elem(name: str, **tensors) -> None:
+    for arg, t in tensors.items():
+        if t is not None and t.dtype not in ELEM:
+            raise NotImplementedError(f"{name}: `{arg}` must be float32, float16 or bfloat16, got {t.dtype}")
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """`_lib.call` with the device's current stream as the last argument, whatever device is current"""
+    fn = getattr(load(), name)
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch.cuda.current_stream(device).cuda_stream), name)
