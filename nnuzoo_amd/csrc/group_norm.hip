@@ -58,9 +58,10 @@ struct GnPlace {
   int col, rr, R;
   bool on;
 };
+template <int NT = GN_NT>
 __device__ __forceinline__ GnPlace gn_place(int cw) {
   GnPlace p;
-  p.R = GN_NT / cw;
+  p.R = NT / cw;
   p.rr = threadIdx.x / cw;
   p.col = threadIdx.x - p.rr * cw;
   p.on = p.rr < p.R;
@@ -68,7 +69,7 @@ __device__ __forceinline__ GnPlace gn_place(int cw) {
 }
 
 // per-channel sums over the workgroup's row threads: v[V] of every thread -> dst[channel], in a fixed order
-template <class A, int V>
+template <class A, int V, int NT = GN_NT>
 __device__ __forceinline__ void gn_fold_rows(A* stage, A* dst, const A (&v)[V], const GnPlace& p, int cw) {
   __syncthreads();
   if (p.on) {
@@ -76,7 +77,7 @@ __device__ __forceinline__ void gn_fold_rows(A* stage, A* dst, const A (&v)[V], 
     for (int j = 0; j < V; ++j) stage[threadIdx.x * V + j] = v[j];
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < cw * V; c += GN_NT) {
+  for (int c = threadIdx.x; c < cw * V; c += NT) {
     A s = 0;
     for (int r = 0; r < p.R; ++r) s += stage[r * cw * V + c];
     dst[c] = s;
@@ -343,6 +344,141 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
   }
 }
 
+// ---- small problems: one launch each way -------------------------------------------------------------------------------------
+// A workgroup owns the C / G channels of a group - of one sample in the forward, of all samples in turn in the backward, whose
+// weight gradients then need no second stage.  Its segments of the rows are short, but everything stays in L2.
+constexpr int GN_SNT = 512;
+// sum over the workgroup of a pair, the same bits in every thread; red: [2 * GN_SNT / 64]
+__device__ __forceinline__ void gn_block_sum(double& s, double& t, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    t += __shfl_xor(t, o, 64);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = s;
+    red[2 * (threadIdx.x >> 6) + 1] = t;
+  }
+  __syncthreads();
+  s = t = 0.0;
+#pragma unroll
+  for (int w = 0; w < GN_SNT / 64; ++w) {
+    s += red[2 * w];
+    t += red[2 * w + 1];
+  }
+}
+
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(GN_SNT) void gn_small_fwd_kernel(GnArgs a) {
+  __shared__ double red[2 * GN_SNT / 64];
+  const long n = blockIdx.x / a.G;
+  const int g = (int)(blockIdx.x - n * a.G), cw = a.q / V;
+  const GnPlace p = gn_place<GN_SNT>(cw);
+  const int c = g * a.q + p.col * V;
+  const TI* x = (const TI*)a.x + n * a.xb + c;
+  double s = 0.0, sq = 0.0;
+  if (p.on) {
+#pragma unroll 4
+    for (long r = p.rr; r < a.S; r += p.R) {
+      float v[V];
+      ld_elems<TI, V>(x + r * a.xs, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double d = (double)v[j];
+        s += d;
+        sq = fma(d, d, sq);
+      }
+    }
+  }
+  gn_block_sum(s, sq, red);
+  const double m = (double)a.S * a.q, mean = s / m;
+  double var = sq / m - mean * mean;
+  if (var < 0.0) var = 0.0;  // NaN stays
+  const float mu = (float)mean, rstd = (float)(1.0 / sqrt(var + (double)a.eps));
+  if (threadIdx.x == 0) {
+    a.stats[(long)blockIdx.x * 2] = mu;
+    a.stats[(long)blockIdx.x * 2 + 1] = rstd;
+  }
+  if (!p.on) return;
+  float w[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = a.w ? a.w[c + j] : 1.f;
+    b[j] = a.b ? a.b[c + j] : 0.f;
+  }
+  TO* y = (TO*)a.out + n * a.S * a.C + c;
+#pragma unroll 4
+  for (long r = p.rr; r < a.S; r += p.R) {
+    float v[V];
+    ld_elems<TI, V>(x + r * a.xs, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = gn_act(fmaf((v[j] - mu) * rstd, w[j], b[j]), a.act, a.slope);
+    st_elems<TO, V>(y + r * a.C, v);
+  }
+}
+
+template <class TI, class TO, int V>
+__global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a) {
+  __shared__ double red[2 * GN_SNT / 64];
+  __shared__ float stage[GN_SNT * V];
+  const int g = blockIdx.x, cw = a.q / V;
+  const GnPlace p = gn_place<GN_SNT>(cw);
+  const int c = g * a.q + p.col * V;
+  float w[V], b[V], sw[V], sb[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    w[j] = a.w && p.on ? a.w[c + j] : 1.f;
+    b[j] = a.b && p.on ? a.b[c + j] : 0.f;
+    sw[j] = sb[j] = 0.f;
+  }
+  const double m = (double)a.S * a.q;
+  for (long n = 0; n < a.N; ++n) {
+    const TI* x = (const TI*)a.x + n * a.xb + c;
+    const TO* dy = (const TO*)a.dy + n * a.S * a.C + c;
+    TI* dx = (TI*)a.out + n * a.S * a.C + c;
+    const float mu = a.stats[(n * a.G + g) * 2], rstd = a.stats[(n * a.G + g) * 2 + 1];
+    double s = 0.0, t = 0.0;
+    if (p.on) {
+#pragma unroll 2
+      for (long r = p.rr; r < a.S; r += p.R) {
+        float v[V], d[V];
+        ld_elems<TI, V>(x + r * a.xs, v);
+        ld_elems<TO, V>(dy + r * a.C, d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = (v[j] - mu) * rstd;
+          const float dz = gn_dact(fmaf(xh, w[j], b[j]), d[j], a.act, a.slope);
+          sb[j] += dz;
+          sw[j] = fmaf(dz, xh, sw[j]);
+          const double wdz = (double)w[j] * dz;
+          s += wdz;
+          t = fma(wdz, (double)xh, t);
+        }
+      }
+    }
+    gn_block_sum(s, t, red);
+    const float m1 = (float)(s / m), m2 = (float)(t / m);
+    if (p.on) {
+#pragma unroll 2
+      for (long r = p.rr; r < a.S; r += p.R) {
+        float v[V], d[V];
+        ld_elems<TI, V>(x + r * a.xs, v);
+        ld_elems<TO, V>(dy + r * a.C, d);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float xh = (v[j] - mu) * rstd;
+          const float dz = gn_dact(fmaf(xh, w[j], b[j]), d[j], a.act, a.slope);
+          v[j] = rstd * (w[j] * dz - m1 - xh * m2);
+        }
+        st_elems<TI, V>(dx + r * a.C, v);
+      }
+    }
+  }
+  if (a.db) gn_fold_rows<float, V, GN_SNT>(stage, a.db + g * a.q, sb, p, cw);
+  if (a.dw) gn_fold_rows<float, V, GN_SNT>(stage, a.dw + g * a.q, sw, p, cw);
+}
+
 constexpr int GN_MAX_C = 4096;    // 2 x C fp64 sums and 256 x V fp64 staging fit LDS
 constexpr long GN_TARGET = 1024;  // workgroups of a launch
 // rows of a workgroup: enough workgroups to fill the chip, at least 8 passes over the rows that its threads cover at once
@@ -356,12 +492,19 @@ inline void gn_split(GnArgs& a, int V) {
   a.rows = (a.S + per - 1) / per;
   a.nblk = (int)((a.S + a.rows - 1) / a.rows);
 }
+// elements of a workgroup up to which the one-launch kernels are taken, samples that the backward may walk in turn
+constexpr long GN_SMALL_FWD = 16384, GN_SMALL_BWD = 32768, GN_SMALL_N = 8;
+inline bool gn_small(long N, long S, int q, bool bwd) {
+  if (q > GN_SNT) return false;
+  return bwd ? N <= GN_SMALL_N && N * S * q <= GN_SMALL_BWD : S * q <= GN_SMALL_FWD;
+}
 inline long gn_align(long v) { return (v + 255) & ~255L; }
 // layout of the workspace, the same whatever V a call's alignment allows
 struct GnWs {
   long gpart, cpart, cc, bytes;
 };
 inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
+  if (gn_small(N, S, C / G, bwd)) return GnWs{};
   long parts = (GN_TARGET + N - 1) / N;   // no split has more parts a sample
   if (parts > S) parts = S;
   GnWs w;
@@ -374,6 +517,13 @@ inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
 
 template <class TI, class TO, int V>
 static int gn_run_fwd(GnArgs a, hipStream_t s) {
+  if (gn_small(a.N, a.S, a.q, false)) {
+    const dim3 small((unsigned)(a.N * a.G));
+    if (a.q % V == 0) NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, V>), small, dim3(GN_SNT), 0, s, a);
+    else NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, 1>), small, dim3(GN_SNT), 0, s, a);
+    NNZ_LAUNCH_CHECK();
+    return NNZ_OK;
+  }
   static DynLdsCache cache;
   gn_split(a, V);
   const int lds = (GN_NT * V + 2 * a.C) * 8;
@@ -390,6 +540,12 @@ static int gn_run_fwd(GnArgs a, hipStream_t s) {
 }
 template <class TI, class TO, int V>
 static int gn_run_bwd(GnArgs a, hipStream_t s) {
+  if (gn_small(a.N, a.S, a.q, true)) {
+    if (a.q % V == 0) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, V>), dim3(a.G), dim3(GN_SNT), 0, s, a);
+    else NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, 1>), dim3(a.G), dim3(GN_SNT), 0, s, a);
+    NNZ_LAUNCH_CHECK();
+    return NNZ_OK;
+  }
   static DynLdsCache cache;
   gn_split(a, V);
   const int lds = (GN_NT * V + 2 * a.C) * 4;
@@ -444,9 +600,9 @@ extern "C" int nnz_group_norm_act_forward(const void* x, int x_type, long x_batc
                                           long workspace_bytes, long N, long S, int C, int G, float eps, int act, float slope,
                                           void* stream) {
   using namespace nnz;
-  if (!x || !y || !stats || !workspace || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
+  if (!x || !y || !stats || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
   const GnWs w = gn_ws(N, S, C, G, false);
-  if (workspace_bytes < w.bytes) return NNZ_EINVAL;
+  if (w.bytes && (!workspace || workspace_bytes < w.bytes)) return NNZ_EINVAL;
   GnArgs a = {};
   a.x = x; a.w = weight; a.b = bias; a.out = y; a.stats = stats; a.gpart = (double*)workspace;
   a.N = N; a.S = S; a.xb = x_batch_stride; a.xs = x_row_stride; a.C = C; a.G = G; a.q = C / G;
@@ -459,9 +615,9 @@ extern "C" int nnz_group_norm_act_backward(const void* x, int x_type, long x_bat
                                            float* dweight, float* dbias, void* workspace, long workspace_bytes, long N, long S,
                                            int C, int G, int act, float slope, void* stream) {
   using namespace nnz;
-  if (!x || !dy || !dx || !stats || !workspace || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
+  if (!x || !dy || !dx || !stats || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
   const GnWs w = gn_ws(N, S, C, G, true);
-  if (workspace_bytes < w.bytes) return NNZ_EINVAL;
+  if (w.bytes && (!workspace || workspace_bytes < w.bytes)) return NNZ_EINVAL;
   GnArgs a = {};
   a.x = x; a.dy = dy; a.w = weight; a.b = bias; a.out = dx; a.stats = (float*)stats;
   a.gpart = (double*)workspace; a.cpart = (float*)((char*)workspace + w.cpart); a.cc = (float*)((char*)workspace + w.cc);

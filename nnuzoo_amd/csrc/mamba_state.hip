@@ -190,15 +190,15 @@ struct ScanStateArgs {
   float* state;          // [B][D][N], batch stride sb, rows contiguous; or null (zeros, nothing kept)
   void* y;               // [B][L][D] contiguous
   const void* len;       // as above
-  float* part_h;         // [chunks][B][D][N]: slot 0 the entry state of the sequence, slot c + 1 the end state of chunk c from a zero
-                         // entry (chunk 0: from the true one)
-  float* part_d;         // [chunks][B][D]: slot c + 1 the sum of D_t over chunk c
+  float* part_h;         // [chunks][B][D][N]: end state of chunk c from a zero entry, then (scan_join_kernel) the true entry state of c
+  float* part_d;         // [chunks][B][D]: sum of D_t over chunk c
   long xb, xt, db, dtt, bb, bt, bg, cb, ct, cg, zb, zt, sb;
   int B, L, D, H, G, softplus, len64, a_n;
   int rep;               // channels of a head
   int dg;                // channels of a group
-  int wpg;               // workgroups (channel blocks) of a group
+  int nch, wpg;          // channels of a workgroup, workgroups of a group
   int cl, chunks;        // tokens of a chunk
+  int pair, pair_dt;     // x and z / dt: two adjacent channels are one aligned access
 };
 
 // e^x with the rounding of x * log2(e) put right
@@ -223,145 +223,235 @@ __device__ __forceinline__ float softplus_hw(float x) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
+// A in units of log 2; an infinite decay becomes a huge one, so that a padding token's D_t = 0 leaves the state alone
+__device__ __forceinline__ float decay2(float A) {
+  const float v = A * LOG2E;
+  return v < -3.0e38f ? -3.0e38f : v;
+}
+// sum over the 4 lanes of a channel (quad_perm: no LDS, unlike a shuffle)
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+  return v;
+}
+template <class T>
+__device__ __forceinline__ float2 ld_pair(const T* p, bool aligned, int second) {
+  if (aligned) {
+    const ElemVec<T, 2> v = *reinterpret_cast<const ElemVec<T, 2>*>(p);
+    return make_float2((float)v[0], (float)v[1]);
+  }
+  return make_float2((float)p[0], (float)p[second]);
+}
 
-// 4 lanes share a channel and hold N / 4 states each; a workgroup has NCH channels of one group and walks its tokens in tiles:
-// every (token, channel) of a tile is loaded and turned into D_t, D_t x_t once, B and C are widened once, all through LDS.
-// MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks: MODE 1 leaves every chunk's summary
-// (end state, sum of D_t: the chunk multiplies its entry state by exp(A sum D)), MODE 2 joins the summaries before its chunk and
-// runs it from the true entry state.
+// 4 lanes share CPL channels and hold N / 4 states of each; a workgroup has nch = 16 CPL channels a wave of one group and walks
+// its tokens in tiles: every (token, channel) of a tile is loaded and turned into D_t, D_t x_t once, B and C are widened once, all
+// through LDS.  Bound by the vector unit: per token, channel and state a 2^x (quarter rate), two products and two FMAs.
+// MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks that run in parallel: MODE 1 leaves
+// every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)),
+// scan_join_kernel turns the summaries into entry states, MODE 2 runs the chunks from those.
 constexpr int SC_TT = 32;   // tokens of a tile
 
-template <class T, int N, int NCH, int MODE>
-__global__ __launch_bounds__(NCH * 4) void scan_prompt_kernel(ScanStateArgs a) {
-  constexpr int NT = NCH * 4, NS = N / 4;
-  constexpr int IT = SC_TT * NCH / NT;   // elements of a thread in the staging passes
-  __shared__ float2 s_du[SC_TT][NCH];
-  __shared__ __attribute__((aligned(16))) float s_b[SC_TT][N];
-  __shared__ __attribute__((aligned(16))) float s_c[SC_TT][N];
-  __shared__ float s_y[SC_TT][NCH];
-  const int tid = threadIdx.x;
+template <class T, int N, int CPL, int MODE>
+__global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
+  constexpr int NS = N / 4;
+  constexpr int IT = CPL == 2 ? 8 : 4;   // token rows of a thread in the staging passes
+  constexpr int ROWS = SC_TT / IT;       // its distance: NT / (nch / 2)
+  extern __shared__ __attribute__((aligned(16))) float sc_lds[];
+  const int nch = a.nch, np = nch / 2;
+  float4* s_du = reinterpret_cast<float4*>(sc_lds);     // [SC_TT][nch / 2]: {D, D x} of two channels
+  float* s_b = sc_lds + SC_TT * nch * 2;                // [SC_TT][N]
+  float* s_c = s_b + SC_TT * N;                         // [SC_TT][N]
+  float* s_y = s_c + SC_TT * N;                         // [SC_TT][nch]
+  const int tid = threadIdx.x, NT = blockDim.x;
   const int g = blockIdx.x / a.wpg;
-  const int ch0 = (blockIdx.x % a.wpg) * NCH;       // within the group
+  const int ch0 = (blockIdx.x - g * a.wpg) * nch;       // within the group
   const int chunk = blockIdx.y, b = blockIdx.z;
   const int len = seq_len(a.len, a.len64, b, a.L);
   const int t0 = chunk * a.cl;
   const int tend = t0 + a.cl < a.L ? t0 + a.cl : a.L;
   const int te = tend < len ? tend : len;
-  // staging role: one channel, tokens (tid / NCH) + 4 i
-  const int sch = tid % NCH, st = tid / NCH;
-  const bool s_on = ch0 + sch < a.dg;
-  const int sd = g * a.dg + (s_on ? ch0 + sch : a.dg - 1);
-  const int shead = sd / a.rep;
-  const float sbias = a.dt_bias ? a.dt_bias[shead] : 0.f;
-  const float sD = a.Dv ? a.Dv[shead] : 0.f;
-  // state role: 4 lanes a channel
-  const int sub = tid & 3, mch = tid >> 2;
-  const bool m_on = ch0 + mch < a.dg;
-  const int md = g * a.dg + (m_on ? ch0 + mch : a.dg - 1);
-  const int mhead = md / a.rep;
-  float A2[NS], h[NS];
-  const long srow = (long)b * a.sb + (long)md * N + sub * NS;
+  // staging role: two adjacent channels, tokens st + ROWS * i
+  const int st = tid / np, sp = tid - st * np;
+  const int sc0 = ch0 + 2 * sp;
+  const bool on0 = sc0 < a.dg, on1 = sc0 + 1 < a.dg;
+  const int sd = g * a.dg + (on0 ? sc0 : a.dg - 1), sd1 = on1 ? 1 : 0;
+  const int hd = sd / a.rep, hd1 = (sd + sd1) / a.rep - hd;
+  const bool pair = a.pair && on1, pair_dt = a.pair_dt && on1;
+  const float bias0 = a.dt_bias ? a.dt_bias[hd] : 0.f, bias1 = a.dt_bias ? a.dt_bias[hd + hd1] : 0.f;
+  const float D0 = a.Dv ? a.Dv[hd] : 0.f, D1 = a.Dv ? a.Dv[hd + hd1] : 0.f;
+  // state role
+  const int sub = tid & 3, mc = (tid >> 2) * CPL;       // the quad's first channel, within the workgroup
+  float A2[CPL][NS], h[CPL][NS];
+  long prow[CPL], srow[CPL];
+  bool m_on[CPL];
 #pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    A2[n] = (a.a_n ? a.A[(long)mhead * N + sub * NS + n] : a.A[mhead]) * LOG2E;
-    h[n] = 0.f;
-  }
-  const long prow = ((long)b * a.D + md) * N + sub * NS, pstep = (long)a.B * a.D * N;
-  if (MODE == 2) {
-    // never from `state`: the workgroup of the last token may have written it already
-    if (t0 < te) {
-      const float* p = a.part_h + (chunk > 0 ? pstep : 0) + prow;
+  for (int q = 0; q < CPL; ++q) {
+    m_on[q] = ch0 + mc + q < a.dg;
+    const int md = g * a.dg + (m_on[q] ? ch0 + mc + q : a.dg - 1), mh = md / a.rep;
+    srow[q] = (long)b * a.sb + (long)md * N + sub * NS;
+    prow[q] = (((long)chunk * a.B + b) * a.D + md) * N + sub * NS;
 #pragma unroll
-      for (int n = 0; n < NS; ++n) h[n] = p[n];
-#pragma unroll 4
-      for (int c = 2; c <= chunk; ++c) {
-        const float sum = a.part_d[((long)c * a.B + b) * a.D + md];
-#pragma unroll
-        for (int n = 0; n < NS; ++n) h[n] = fmaf(__builtin_amdgcn_exp2f(sum * A2[n]), h[n], a.part_h[c * pstep + prow + n]);
-      }
+    for (int n = 0; n < NS; ++n) {
+      A2[q][n] = decay2(a.a_n ? a.A[(long)mh * N + sub * NS + n] : a.A[mh]);
+      h[q][n] = MODE == 2 ? a.part_h[prow[q] + n] : MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
     }
-  } else if (chunk == 0 && a.state) {
-#pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = a.state[srow + n];
   }
-  if (MODE == 1 && chunk == 0 && m_on) {
-#pragma unroll
-    for (int n = 0; n < NS; ++n) a.part_h[prow + n] = h[n];
-  }
-  float dsum = 0.f;
+  float dsum[CPL] = {};
   const T* xp = (const T*)a.x + (long)b * a.xb + sd;
   const T* zp = a.z ? (const T*)a.z + (long)b * a.zb + sd : nullptr;
-  const T* dp = (const T*)a.dt + (long)b * a.db + shead;
+  const T* dp = (const T*)a.dt + (long)b * a.db + hd;
   const T* bp = (const T*)a.Bm + (long)b * a.bb + g * a.bg;
   const T* cp = (const T*)a.Cm + (long)b * a.cb + g * a.cg;
   T* yp = (T*)a.y + (long)b * a.L * a.D + sd;
   for (int tile = t0; tile < te; tile += SC_TT) {
-    float xv[IT], zv[IT];
+    float2 xv[IT], zv[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int t = tile + st + 4 * i;
-      float dl = 0.f;
-      xv[i] = 0.f;
-      zv[i] = 0.f;
+      const int t = tile + st + ROWS * i;
+      float2 dl = make_float2(0.f, 0.f);
+      xv[i] = zv[i] = dl;
       if (t < te) {
-        xv[i] = (float)xp[(long)t * a.xt];
-        if (MODE != 1 && zp) zv[i] = (float)zp[(long)t * a.zt];
-        dl = (float)dp[(long)t * a.dtt] + sbias;
-        if (a.softplus) dl = softplus_hw(dl);
+        xv[i] = ld_pair<T>(xp + (long)t * a.xt, pair, sd1);
+        if (MODE != 1 && zp) zv[i] = ld_pair<T>(zp + (long)t * a.zt, pair, sd1);
+        dl = ld_pair<T>(dp + (long)t * a.dtt, pair_dt, hd1);
+        dl.x += bias0;
+        dl.y += bias1;
+        if (a.softplus) {
+          dl.x = softplus_hw(dl.x);
+          dl.y = softplus_hw(dl.y);
+        }
       }
-      s_du[st + 4 * i][sch] = make_float2(dl, dl * xv[i]);
+      s_du[(st + ROWS * i) * np + sp] = make_float4(dl.x, dl.x * xv[i].x, dl.y, dl.y * xv[i].y);
     }
     for (int i = tid; i < SC_TT * N; i += NT) {
       const int tt = i / N, n = i % N, t = tile + tt;
-      s_b[tt][n] = t < te ? (float)bp[(long)t * a.bt + n] : 0.f;
-      if (MODE != 1) s_c[tt][n] = t < te ? (float)cp[(long)t * a.ct + n] : 0.f;
+      s_b[i] = t < te ? (float)bp[(long)t * a.bt + n] : 0.f;
+      if (MODE != 1) s_c[i] = t < te ? (float)cp[(long)t * a.ct + n] : 0.f;
     }
     __syncthreads();
     const int cnt = te - tile < SC_TT ? te - tile : SC_TT;
-#pragma unroll 4
-    for (int tt = 0; tt < cnt; ++tt) {
-      const float2 du = s_du[tt][mch];
-      float acc = 0.f;
+    // 4 tokens at a time; a tile's tokens behind the end have D = 0 and change nothing
+    for (int tt = 0; tt < cnt; tt += 4) {
+      float yv[CPL];
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        h[n] = fmaf(__builtin_amdgcn_exp2f(du.x * A2[n]), h[n], du.y * s_b[tt][sub * NS + n]);
-        if (MODE != 1) acc = fmaf(h[n], s_c[tt][sub * NS + n], acc);
+      for (int k = 0; k < 4; ++k) {
+        float d[CPL], u[CPL];
+        if constexpr (CPL == 2) {
+          const float4 v = s_du[(tt + k) * np + (mc >> 1)];
+          d[0] = v.x; u[0] = v.y; d[1] = v.z; u[1] = v.w;
+        } else {
+          const float2 v = reinterpret_cast<const float2*>(s_du)[(tt + k) * nch + mc];
+          d[0] = v.x; u[0] = v.y;
+        }
+        float bv[NS], cv[NS];
+        ld_elems<float, NS>(s_b + (tt + k) * N + sub * NS, bv);
+        if (MODE != 1) ld_elems<float, NS>(s_c + (tt + k) * N + sub * NS, cv);
+#pragma unroll
+        for (int q = 0; q < CPL; ++q) {
+          float acc = 0.f;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            h[q][n] = fmaf(__builtin_amdgcn_exp2f(d[q] * A2[q][n]), h[q][n], u[q] * bv[n]);
+            if (MODE != 1) acc = n ? fmaf(h[q][n], cv[n], acc) : h[q][n] * cv[n];
+          }
+          if (MODE == 1) dsum[q] += d[q];
+          else {
+            acc = quad_sum(acc);
+            yv[q] = k == 0 || sub == k ? acc : yv[q];   // lane k of the quad keeps token k
+          }
+        }
       }
-      if (MODE == 1) dsum += du.x;
-      else {
-        acc += __shfl_xor(acc, 1, 64);
-        acc += __shfl_xor(acc, 2, 64);
-        if (sub == 0) s_y[tt][mch] = acc;
+      if (MODE != 1) {
+        if constexpr (CPL == 2) *reinterpret_cast<float2*>(s_y + (tt + sub) * nch + mc) = make_float2(yv[0], yv[1]);
+        else s_y[(tt + sub) * nch + mc] = yv[0];
       }
     }
     __syncthreads();
     if (MODE != 1) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const int t = tile + st + 4 * i;
-        if (t < te && s_on) {
-          float v = fmaf(sD, xv[i], s_y[st + 4 * i][sch]);
-          if (zp) v *= zv[i] * sigmoid_hw(zv[i]);
-          yp[(long)t * a.D] = (T)v;
+        const int tt = st + ROWS * i, t = tile + tt;
+        if (t < te && on0) {
+          const float2 yy = *reinterpret_cast<const float2*>(s_y + tt * nch + 2 * sp);
+          float v0 = fmaf(D0, xv[i].x, yy.x), v1 = fmaf(D1, xv[i].y, yy.y);
+          if (zp) {
+            v0 *= zv[i].x * sigmoid_hw(zv[i].x);
+            v1 *= zv[i].y * sigmoid_hw(zv[i].y);
+          }
+          T* o = yp + (long)t * a.D;
+          if (pair) {
+            ElemVec<T, 2> r;
+            r[0] = (T)v0;
+            r[1] = (T)v1;
+            *reinterpret_cast<ElemVec<T, 2>*>(o) = r;
+          } else {
+            o[0] = (T)v0;
+            if (on1) o[1] = (T)v1;
+          }
         }
       }
     }
   }
   if (MODE == 1) {
-    if (m_on) {
-      float* o = a.part_h + (chunk + 1) * pstep + prow;
 #pragma unroll
-      for (int n = 0; n < NS; ++n) o[n] = h[n];
-      if (sub == 0) a.part_d[((long)(chunk + 1) * a.B + b) * a.D + md] = dsum;
-    }
+    for (int q = 0; q < CPL; ++q)
+      if (m_on[q]) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) a.part_h[prow[q] + n] = h[q][n];
+        if (sub == 0) a.part_d[prow[q] / N] = dsum[q];
+      }
     return;
   }
-  if (s_on)
-    for (int t = (te > t0 ? te : t0) + st; t < tend; t += 4) yp[(long)t * a.D] = (T)0.f;
-  // the chunk that holds the last token leaves the state
-  if (a.state && m_on && len > 0 && t0 < len && len <= tend) {
+  if (on0)
+    for (int t = (te > t0 ? te : t0) + st; t < tend; t += ROWS) {
+      yp[(long)t * a.D] = (T)0.f;
+      if (on1) yp[(long)t * a.D + 1] = (T)0.f;
+    }
+  // the chunk that holds the last token leaves the state (chunks read `state` in scan_join_kernel only)
+  if (a.state && len > t0 && len <= tend) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) a.state[srow + n] = h[n];
+    for (int q = 0; q < CPL; ++q)
+      if (m_on[q]) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) a.state[srow[q] + n] = h[q][n];
+      }
+  }
+}
+
+// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A lane per (channel, state), 8 waves
+// share the chunks: each joins its own run of them, then starts again from the runs before it.
+constexpr int SJ_SEG = 8;
+template <int N>
+__global__ __launch_bounds__(64 * SJ_SEG) void scan_join_kernel(ScanStateArgs a) {
+  __shared__ float s_p[SJ_SEG][64], s_h[SJ_SEG][64];
+  const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6, b = blockIdx.y;
+  const long dn = (long)a.D * N, i = (long)blockIdx.x * 64 + lane;
+  const long at = i < dn ? i : dn - 1;
+  const int d = (int)(at / N), hd = d / a.rep;
+  const float A2 = decay2(a.a_n ? a.A[(long)hd * N + at % N] : a.A[hd]);
+  const int per = (a.chunks + SJ_SEG - 1) / SJ_SEG;
+  const int c0 = seg * per, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
+  float* ph = a.part_h + (long)b * dn + at;
+  const float* pd = a.part_d + (long)b * a.D + d;
+  const long hs = (long)a.B * dn, ds = (long)a.B * a.D;
+  float p = 0.f, h = 0.f;
+#pragma unroll 8
+  for (int c = c0; c < c1; ++c) {
+    const float sum = pd[c * ds];
+    h = fmaf(__builtin_amdgcn_exp2f(sum * A2), h, ph[c * hs]);
+    p += sum;
+  }
+  s_p[seg][lane] = p;
+  s_h[seg][lane] = h;
+  __syncthreads();
+  float e = a.state ? a.state[(long)b * a.sb + at] : 0.f;
+  for (int s = 0; s < seg; ++s) e = fmaf(__builtin_amdgcn_exp2f(s_p[s][lane] * A2), e, s_h[s][lane]);
+  if (i >= dn) return;
+#pragma unroll 8
+  for (int c = c0; c < c1; ++c) {
+    const float own = ph[c * hs], sum = pd[c * ds];
+    ph[c * hs] = e;
+    e = fmaf(__builtin_amdgcn_exp2f(sum * A2), e, own);
   }
 }
 
@@ -389,13 +479,12 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
   float acc = 0.f;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    const float A2 = (a.a_n ? a.A[(long)head * N + sub * NS + n] : a.A[head]) * LOG2E;
+    const float A2 = decay2(a.a_n ? a.A[(long)head * N + sub * NS + n] : a.A[head]);
     const float h = fmaf(__builtin_amdgcn_exp2f(dl * A2), st[n], u * (float)bp[n]);
     st[n] = h;
     acc = fmaf(h, (float)cp[n], acc);
   }
-  acc += __shfl_xor(acc, 1, 64);
-  acc += __shfl_xor(acc, 2, 64);
+  acc = quad_sum(acc);
   if (sub == 0) {
     float v = a.Dv ? fmaf(a.Dv[head], x, acc) : acc;
     if (a.z) {
@@ -407,52 +496,57 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
-constexpr int SC_MAX_CHUNKS = 128;
-// channels of a workgroup: the widest block that pads the group's channels least
-inline int scan_nch(int dg) {
-  int best = 16;
-  for (int c = 32; c <= 64; c *= 2)
-    if ((dg + c - 1) / c * c <= (dg + best - 1) / best * best) best = c;
-  return best;
-}
 struct ScanSplit {
-  int nch, wpg, cl, chunks;
+  int cpl, nch, wpg, cl, chunks;
 };
-// Chunks cost a second pass over the states, so sequences are cut only where whole ones leave most of the chip idle
-// (256 CUs x 4 SIMDs: under 512 waves), into chunks of at least 4 tiles, until there are about 2 048 waves.
+// Chunks cost a second pass over the states, so sequences are cut only where whole ones leave most of the chip idle: into chunks of
+// at least 64 tokens until there are about 4 096 waves (4 a SIMD), and only if that makes at least 4 of them.
+// Two channels a quad (half the LDS reads of B and C) once there are enough waves; one where the latency of few waves counts.
 inline ScanSplit scan_split(int B, int L, int D, int G) {
   ScanSplit s;
   const int dg = D / G;
-  s.nch = scan_nch(dg);
-  s.wpg = (dg + s.nch - 1) / s.nch;
-  const long waves = (long)B * G * s.wpg * (s.nch / 16);
-  long want = waves >= 512 ? 1 : (2048 + waves - 1) / waves;
-  const long most = (L + 4 * SC_TT - 1) / (4 * SC_TT);
+  const long waves2 = (long)B * G * ((dg + 31) / 32);
+  long want = 4096 / waves2;
+  const long most = (L + 63) / 64;
   if (want > most) want = most;
-  if (want > SC_MAX_CHUNKS) want = SC_MAX_CHUNKS;
-  if (want < 1) want = 1;
+  if (want < 4) want = 1;
+  s.cpl = waves2 * want >= 512 ? 2 : 1;
   long cl = (L + want - 1) / want;
   cl = (cl + SC_TT - 1) / SC_TT * SC_TT;
   s.cl = (int)cl;
   s.chunks = (int)((L + cl - 1) / cl);
+  // up to 4 waves a workgroup, as many as pad the group's channels least
+  const int wch = 16 * s.cpl, need = (dg + wch - 1) / wch;
+  int best = 1;
+  for (int w = 2; w <= 4; ++w)
+    if ((need + w - 1) / w * w <= (need + best - 1) / best * best) best = w;
+  s.nch = best * wch;
+  s.wpg = (dg + s.nch - 1) / s.nch;
   return s;
 }
-template <class T, int N, int NCH>
+template <class T, int N, int CPL>
 static int scan_prompt_run(const ScanStateArgs& a, hipStream_t s) {
-  const dim3 grid(a.G * a.wpg, a.chunks, a.B);
+  const dim3 grid(a.G * a.wpg, a.chunks, a.B), block(a.nch * 4 / CPL);
+  const int lds = SC_TT * (3 * a.nch + 2 * N) * 4;
+  static DynLdsCache c0, c1, c2;
+  hipError_t e;
   if (a.chunks == 1) {
-    NNZ_LAUNCH((scan_prompt_kernel<T, N, NCH, 0>), grid, dim3(NCH * 4), 0, s, a);
+    if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 0>, lds, c0)) != hipSuccess) return (int)e;
+    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 0>), grid, block, lds, s, a);
   } else {
-    // the last chunk's summary is not needed
-    NNZ_LAUNCH((scan_prompt_kernel<T, N, NCH, 1>), dim3(a.G * a.wpg, a.chunks - 1, a.B), dim3(NCH * 4), 0, s, a);
+    if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 1>, lds, c1)) != hipSuccess) return (int)e;
+    if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 2>, lds, c2)) != hipSuccess) return (int)e;
+    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), grid, block, lds, s, a);
     NNZ_LAUNCH_CHECK();
-    NNZ_LAUNCH((scan_prompt_kernel<T, N, NCH, 2>), grid, dim3(NCH * 4), 0, s, a);
+    NNZ_LAUNCH((scan_join_kernel<N>), dim3((unsigned)(((long)a.D * N + 63) / 64), a.B), dim3(64 * SJ_SEG), 0, s, a);
+    NNZ_LAUNCH_CHECK();
+    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 2>), grid, block, lds, s, a);
   }
   NNZ_LAUNCH_CHECK();
   return NNZ_OK;
 }
 template <class T, int N>
-static int scan_state_run(const ScanStateArgs& a, int nch, bool token, hipStream_t s) {
+static int scan_state_run(const ScanStateArgs& a, int cpl, bool token, hipStream_t s) {
   if (token) {
     const long wg = ((long)a.B * a.D * 4 + 255) / 256;
     if (wg > 0x7FFFFFFFL) return NNZ_EINVAL;
@@ -460,24 +554,22 @@ static int scan_state_run(const ScanStateArgs& a, int nch, bool token, hipStream
     NNZ_LAUNCH_CHECK();
     return NNZ_OK;
   }
-  if (nch == 64) return scan_prompt_run<T, N, 64>(a, s);
-  if (nch == 32) return scan_prompt_run<T, N, 32>(a, s);
-  return scan_prompt_run<T, N, 16>(a, s);
+  return cpl == 2 ? scan_prompt_run<T, N, 2>(a, s) : scan_prompt_run<T, N, 1>(a, s);
 }
 template <class T>
-static int scan_state_n(const ScanStateArgs& a, int N, int nch, bool token, hipStream_t s) {
+static int scan_state_n(const ScanStateArgs& a, int N, int cpl, bool token, hipStream_t s) {
   switch (N) {
-    case 4: return scan_state_run<T, 4>(a, nch, token, s);
-    case 8: return scan_state_run<T, 8>(a, nch, token, s);
-    case 16: return scan_state_run<T, 16>(a, nch, token, s);
-    case 32: return scan_state_run<T, 32>(a, nch, token, s);
+    case 4: return scan_state_run<T, 4>(a, cpl, token, s);
+    case 8: return scan_state_run<T, 8>(a, cpl, token, s);
+    case 16: return scan_state_run<T, 16>(a, cpl, token, s);
+    case 32: return scan_state_run<T, 32>(a, cpl, token, s);
   }
   return NNZ_EINVAL;
 }
-static int scan_state_go(const ScanStateArgs& a, int type, int N, int nch, bool token, hipStream_t s) {
-  if (type == ELEM_F32) return scan_state_n<float>(a, N, nch, token, s);
-  if (type == ELEM_F16) return scan_state_n<f16>(a, N, nch, token, s);
-  if (type == ELEM_BF16) return scan_state_n<bf16>(a, N, nch, token, s);
+static int scan_state_go(const ScanStateArgs& a, int type, int N, int cpl, bool token, hipStream_t s) {
+  if (type == ELEM_F32) return scan_state_n<float>(a, N, cpl, token, s);
+  if (type == ELEM_F16) return scan_state_n<f16>(a, N, cpl, token, s);
+  if (type == ELEM_BF16) return scan_state_n<bf16>(a, N, cpl, token, s);
   return NNZ_EINVAL;
 }
 static bool scan_shape_ok(int B, int L, int D, int H, int G, int N) {
@@ -538,8 +630,11 @@ extern "C" int nnz_selective_scan_prompt(const void* x, const void* dt, const vo
   a.part_h = (float*)workspace;
   a.part_d = a.part_h + (long)sp.chunks * B * D * N;
   a.B = B; a.L = L; a.D = D; a.H = H; a.G = G; a.softplus = softplus;
-  a.rep = D / H; a.dg = D / G; a.wpg = sp.wpg; a.cl = sp.cl; a.chunks = sp.chunks;
-  return scan_state_go(a, type, N, sp.nch, false, (hipStream_t)stream);
+  a.rep = D / H; a.dg = D / G; a.nch = sp.nch; a.wpg = sp.wpg; a.cl = sp.cl; a.chunks = sp.chunks;
+  const uintptr_t m = 2 * (uintptr_t)elem_size(type) - 1;   // a pair's alignment; a group begins at an even channel
+  a.pair = (((uintptr_t)x | (uintptr_t)z | (uintptr_t)y) & m) == 0 && ((a.xb | a.xt | a.zb | a.zt | D | a.dg) & 1) == 0;
+  a.pair_dt = a.rep == 1 && ((uintptr_t)dt & m) == 0 && ((a.db | a.dtt | a.dg) & 1) == 0;
+  return scan_state_go(a, type, N, sp.cpl, false, (hipStream_t)stream);
 }
 
 extern "C" int nnz_selective_scan_token(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,

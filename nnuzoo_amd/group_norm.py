@@ -48,16 +48,15 @@ class _GroupNormActFn(torch.autograd.Function):
         N, C = x.shape[0], x.shape[-1]
         y = torch.empty(x.shape, dtype=out_dtype, device=dev)
         ctx.cfg = (xb, xs, groups, act, slope)
-        ctx.affine = (weight is not None, bias is not None)
         if y.numel() == 0:
             ctx.save_for_backward(x, weight, bias, None)
             return y
         S = x.numel() // (N * C)
         ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 0)
-        ws = torch.empty(max(ws_bytes, 0), dtype=torch.uint8, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         stats = torch.empty(2 * N * groups, dtype=torch.float32, device=dev)
         launch("nnz_group_norm_act_forward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, ptr(weight), ptr(bias), y.data_ptr(),
-               ELEM[out_dtype], stats.data_ptr(), ws.data_ptr(), ws_bytes, N, S, C, groups, eps, act, slope)
+               ELEM[out_dtype], stats.data_ptr(), ptr(ws), ws_bytes, N, S, C, groups, eps, act, slope)
         ctx.save_for_backward(x, weight, bias, stats)
         return y
 
@@ -70,15 +69,15 @@ class _GroupNormActFn(torch.autograd.Function):
         need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         make = torch.empty if stats is not None else torch.zeros
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        affine = make((2, C), dtype=torch.float32, device=dev) if need_w or need_b else None
-        dw, db = (affine[0] if need_w else None), (affine[1] if need_b else None)
+        dw = make(C, dtype=torch.float32, device=dev) if need_w else None
+        db = make(C, dtype=torch.float32, device=dev) if need_b else None
         if stats is not None:
             dy = dy.contiguous()
             S = x.numel() // (N * C)
             ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
-            ws = torch.empty(max(ws_bytes, 0), dtype=torch.uint8, device=dev)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
             launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
-                   ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ws.data_ptr(), ws_bytes, N, S, C,
+                   ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C,
                    groups, act, slope)
         return dx, dw, db, None, None, None, None, None
 
