@@ -8,6 +8,8 @@
 // Sums and states are fp32 whatever the activations' type.
 #include "elem_io.hpp"
 
+#include <type_traits>
+
 namespace nnz {
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -208,18 +210,14 @@ __device__ __forceinline__ float exp_fine(float x) {
   const float e = __builtin_amdgcn_exp2f(p);
   return fmaf(e * 0.6931471805599453f, r, e);
 }
-// softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|) <= 1, by log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1/3: relative accuracy
-// for small e, too (a time step is often softplus of -5, and the states' decay takes its relative error)
+// softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|) <= 1; w = 1 + e is rounded, and what the rounding lost is added to log w
+// (v_log_f32 keeps 1 ulp of its result down to w = 1 + 2^-23): relative accuracy for small e, too - a time step is often softplus of
+// -5, and the states' decay takes its relative error.  e is 0 beyond -110.
 __device__ __forceinline__ float softplus_hw(float x) {
-  const float e = x == x ? exp_fine(-fabsf(x)) : x;
-  const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-  float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-  p = fmaf(q, p, 1.f / 9.f);
-  p = fmaf(q, p, 1.f / 7.f);
-  p = fmaf(q, p, 1.f / 5.f);
-  p = fmaf(q, p, 1.f / 3.f);
-  p = fmaf(q, p, 1.f);
-  return fmaf(2.f * s, p, x > 0.f ? x : 0.f);
+  const float e = exp_fine(-fminf(fabsf(x), 110.f));
+  const float w = 1.f + e;
+  const float l = fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, e - (w - 1.f));
+  return l + (x < 0.f ? 0.f : x);   // NaN stays
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -235,12 +233,9 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v;
 }
 template <class T>
-__device__ __forceinline__ float2 ld_pair(const T* p, bool aligned, int second) {
-  if (aligned) {
-    const ElemVec<T, 2> v = *reinterpret_cast<const ElemVec<T, 2>*>(p);
-    return make_float2((float)v[0], (float)v[1]);
-  }
-  return make_float2((float)p[0], (float)p[second]);
+__device__ __forceinline__ ElemVec<T, 2> ld_pair(const T* p, bool aligned, int second) {
+  if (aligned) return *reinterpret_cast<const ElemVec<T, 2>*>(p);
+  return ElemVec<T, 2>{p[0], p[second]};
 }
 
 // 4 lanes share CPL channels and hold N / 4 states of each; a workgroup has nch = 16 CPL channels a wave of one group and walks
@@ -249,19 +244,19 @@ __device__ __forceinline__ float2 ld_pair(const T* p, bool aligned, int second) 
 // MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks that run in parallel: MODE 1 leaves
 // every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)),
 // scan_join_kernel turns the summaries into entry states, MODE 2 runs the chunks from those.
-constexpr int SC_TT = 32;   // tokens of a tile
+constexpr int SC_TT = 16;   // tokens of a tile
 
 template <class T, int N, int CPL, int MODE>
 __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
   constexpr int NS = N / 4;
-  constexpr int IT = CPL == 2 ? 8 : 4;   // token rows of a thread in the staging passes
+  constexpr int IT = SC_TT * CPL / 8;    // token rows of a thread in the staging passes
   constexpr int ROWS = SC_TT / IT;       // its distance: NT / (nch / 2)
   extern __shared__ __attribute__((aligned(16))) float sc_lds[];
   const int nch = a.nch, np = nch / 2;
   float4* s_du = reinterpret_cast<float4*>(sc_lds);     // [SC_TT][nch / 2]: {D, D x} of two channels
   float* s_b = sc_lds + SC_TT * nch * 2;                // [SC_TT][N]
-  float* s_c = s_b + SC_TT * N;                         // [SC_TT][N]
-  float* s_y = s_c + SC_TT * N;                         // [SC_TT][nch]
+  float* s_c = s_b + SC_TT * N;                         // [SC_TT][N], not in MODE 1
+  float* s_y = s_c + SC_TT * N;                         // [SC_TT][nch], not in MODE 1
   const int tid = threadIdx.x, NT = blockDim.x;
   const int g = blockIdx.x / a.wpg;
   const int ch0 = (blockIdx.x - g * a.wpg) * nch;       // within the group
@@ -297,67 +292,127 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
     }
   }
   float dsum[CPL] = {};
-  const T* xp = (const T*)a.x + (long)b * a.xb + sd;
-  const T* zp = a.z ? (const T*)a.z + (long)b * a.zb + sd : nullptr;
-  const T* dp = (const T*)a.dt + (long)b * a.db + hd;
-  const T* bp = (const T*)a.Bm + (long)b * a.bb + g * a.bg;
-  const T* cp = (const T*)a.Cm + (long)b * a.cb + g * a.cg;
-  T* yp = (T*)a.y + (long)b * a.L * a.D + sd;
+  // every access walks its rows by a constant step
+  const T* xp = (const T*)a.x + (long)b * a.xb + (long)(t0 + st) * a.xt + sd;
+  const T* zp = (const T*)a.z + (a.z ? (long)b * a.zb + (long)(t0 + st) * a.zt + sd : 0);
+  const T* dp = (const T*)a.dt + (long)b * a.db + (long)(t0 + st) * a.dtt + hd;
+  T* yp = (T*)a.y + ((long)b * a.L + t0 + st) * a.D + sd;
+  const int bn = tid % N, b0 = tid / N, brows = NT / N;   // N <= 32 divides NT
+  const T* bp = (const T*)a.Bm + (long)b * a.bb + g * a.bg + (long)(t0 + b0) * a.bt + bn;
+  const T* cp = (const T*)a.Cm + (long)b * a.cb + g * a.cg + (long)(t0 + b0) * a.ct + bn;
+  const long xs = ROWS * a.xt, zs = ROWS * a.zt, dls = ROWS * a.dtt, ys = (long)ROWS * a.D;
+  // a tile's loads are issued before the tile in front of it is computed
+  constexpr int BI = SC_TT * N / 64;
+  typedef ElemVec<T, 2> Pair;
+  Pair xr[IT], zr[IT], dr[IT];
+  T br[BI], cr[BI];
+  const Pair none = {(T)0.f, (T)0.f};
+  auto fetch_rows = [&](int tile, auto whole) __attribute__((always_inline)) {
+    constexpr bool W = decltype(whole)::value;   // all rows of the tile exist
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const bool in = W || tile + st + ROWS * i < te;
+      xr[i] = in ? ld_pair<T>(xp, pair, sd1) : none;
+      dr[i] = in ? ld_pair<T>(dp, pair_dt, hd1) : none;
+      if (MODE != 1) zr[i] = in && a.z ? ld_pair<T>(zp, pair, sd1) : none;
+      xp += xs;
+      dp += dls;
+      if (MODE != 1) zp += zs;
+    }
+#pragma unroll
+    for (int i = 0; i < BI; ++i) {
+      const int tt = b0 + i * brows;
+      const bool in = tt < SC_TT && (W || tile + tt < te);
+      br[i] = in ? bp[(long)i * brows * a.bt] : (T)0.f;
+      if (MODE != 1) cr[i] = in ? cp[(long)i * brows * a.ct] : (T)0.f;
+    }
+    bp += SC_TT * a.bt;
+    cp += SC_TT * a.ct;
+  };
+  auto fetch = [&](int tile) __attribute__((always_inline)) {
+    if (tile + SC_TT <= te) fetch_rows(tile, std::true_type{});
+    else fetch_rows(tile, std::false_type{});
+  };
+  if (t0 < te) fetch(t0);
   for (int tile = t0; tile < te; tile += SC_TT) {
     float2 xv[IT], zv[IT];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int t = tile + st + ROWS * i;
-      float2 dl = make_float2(0.f, 0.f);
-      xv[i] = zv[i] = dl;
-      if (t < te) {
-        xv[i] = ld_pair<T>(xp + (long)t * a.xt, pair, sd1);
-        if (MODE != 1 && zp) zv[i] = ld_pair<T>(zp + (long)t * a.zt, pair, sd1);
-        dl = ld_pair<T>(dp + (long)t * a.dtt, pair_dt, hd1);
-        dl.x += bias0;
-        dl.y += bias1;
-        if (a.softplus) {
-          dl.x = softplus_hw(dl.x);
-          dl.y = softplus_hw(dl.y);
-        }
+      xv[i] = make_float2((float)xr[i][0], (float)xr[i][1]);
+      if (MODE != 1) zv[i] = make_float2((float)zr[i][0], (float)zr[i][1]);
+      float dl0 = (float)dr[i][0] + bias0, dl1 = (float)dr[i][1] + bias1;
+      if (a.softplus) {
+        dl0 = softplus_hw(dl0);
+        dl1 = softplus_hw(dl1);
       }
-      s_du[(st + ROWS * i) * np + sp] = make_float4(dl.x, dl.x * xv[i].x, dl.y, dl.y * xv[i].y);
+      if (tile + st + ROWS * i >= te) dl0 = dl1 = 0.f;
+      s_du[(st + ROWS * i) * np + sp] = make_float4(dl0, dl0 * xv[i].x, dl1, dl1 * xv[i].y);
     }
-    for (int i = tid; i < SC_TT * N; i += NT) {
-      const int tt = i / N, n = i % N, t = tile + tt;
-      s_b[i] = t < te ? (float)bp[(long)t * a.bt + n] : 0.f;
-      if (MODE != 1) s_c[i] = t < te ? (float)cp[(long)t * a.ct + n] : 0.f;
+#pragma unroll
+    for (int i = 0; i < BI; ++i) {
+      const int tt = b0 + i * brows;
+      if (tt < SC_TT) {
+        s_b[tt * N + bn] = (float)br[i];
+        if (MODE != 1) s_c[tt * N + bn] = (float)cr[i];
+      }
     }
+    if (tile + SC_TT < te) fetch(tile + SC_TT);
     __syncthreads();
     const int cnt = te - tile < SC_TT ? te - tile : SC_TT;
     // 4 tokens at a time; a tile's tokens behind the end have D = 0 and change nothing
     for (int tt = 0; tt < cnt; tt += 4) {
       float yv[CPL];
+      if constexpr (CPL == 1) {
+        // few waves: 4 tokens' reads and decays before their recurrence, so that the latencies overlap
+        float d[4], u[4], bv[4][NS], cv[4][NS], e[4][NS];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float d[CPL], u[CPL];
-        if constexpr (CPL == 2) {
-          const float4 v = s_du[(tt + k) * np + (mc >> 1)];
-          d[0] = v.x; u[0] = v.y; d[1] = v.z; u[1] = v.w;
-        } else {
+        for (int k = 0; k < 4; ++k) {
           const float2 v = reinterpret_cast<const float2*>(s_du)[(tt + k) * nch + mc];
-          d[0] = v.x; u[0] = v.y;
+          d[k] = v.x;
+          u[k] = v.y;
+          ld_elems<float, NS>(s_b + (tt + k) * N + sub * NS, bv[k]);
+          if (MODE != 1) ld_elems<float, NS>(s_c + (tt + k) * N + sub * NS, cv[k]);
         }
-        float bv[NS], cv[NS];
-        ld_elems<float, NS>(s_b + (tt + k) * N + sub * NS, bv);
-        if (MODE != 1) ld_elems<float, NS>(s_c + (tt + k) * N + sub * NS, cv);
 #pragma unroll
-        for (int q = 0; q < CPL; ++q) {
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int n = 0; n < NS; ++n) e[k][n] = __builtin_amdgcn_exp2f(d[k] * A2[0][n]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
           float acc = 0.f;
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            h[q][n] = fmaf(__builtin_amdgcn_exp2f(d[q] * A2[q][n]), h[q][n], u[q] * bv[n]);
-            if (MODE != 1) acc = n ? fmaf(h[q][n], cv[n], acc) : h[q][n] * cv[n];
+            h[0][n] = fmaf(e[k][n], h[0][n], u[k] * bv[k][n]);
+            if (MODE != 1) acc = n ? fmaf(h[0][n], cv[k][n], acc) : h[0][n] * cv[k][n];
           }
-          if (MODE == 1) dsum[q] += d[q];
+          if (MODE == 1) dsum[0] += d[k];
           else {
             acc = quad_sum(acc);
-            yv[q] = k == 0 || sub == k ? acc : yv[q];   // lane k of the quad keeps token k
+            yv[0] = k == 0 || sub == k ? acc : yv[0];   // lane k of the quad keeps token k
+          }
+        }
+      } else {
+        // many waves hide the latencies, and registers count
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 v = s_du[(tt + k) * np + (mc >> 1)];
+          const float d[2] = {v.x, v.z}, u[2] = {v.y, v.w};
+          float bv[NS], cv[NS];
+          ld_elems<float, NS>(s_b + (tt + k) * N + sub * NS, bv);
+          if (MODE != 1) ld_elems<float, NS>(s_c + (tt + k) * N + sub * NS, cv);
+#pragma unroll
+          for (int q = 0; q < CPL; ++q) {
+            float acc = 0.f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+              h[q][n] = fmaf(__builtin_amdgcn_exp2f(d[q] * A2[q][n]), h[q][n], u[q] * bv[n]);
+              if (MODE != 1) acc = n ? fmaf(h[q][n], cv[n], acc) : h[q][n] * cv[n];
+            }
+            if (MODE == 1) dsum[q] += d[q];
+            else {
+              acc = quad_sum(acc);
+              yv[q] = k == 0 || sub == k ? acc : yv[q];
+            }
           }
         }
       }
@@ -374,11 +429,11 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
         if (t < te && on0) {
           const float2 yy = *reinterpret_cast<const float2*>(s_y + tt * nch + 2 * sp);
           float v0 = fmaf(D0, xv[i].x, yy.x), v1 = fmaf(D1, xv[i].y, yy.y);
-          if (zp) {
+          if (a.z) {
             v0 *= zv[i].x * sigmoid_hw(zv[i].x);
             v1 *= zv[i].y * sigmoid_hw(zv[i].y);
           }
-          T* o = yp + (long)t * a.D;
+          T* o = yp + i * ys;
           if (pair) {
             ElemVec<T, 2> r;
             r[0] = (T)v0;
@@ -390,6 +445,7 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
           }
         }
       }
+      yp += IT * ys;
     }
   }
   if (MODE == 1) {
@@ -402,11 +458,13 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
       }
     return;
   }
-  if (on0)
+  if (on0) {
+    T* y0 = (T*)a.y + (long)b * a.L * a.D + sd;
     for (int t = (te > t0 ? te : t0) + st; t < tend; t += ROWS) {
-      yp[(long)t * a.D] = (T)0.f;
-      if (on1) yp[(long)t * a.D + 1] = (T)0.f;
+      y0[(long)t * a.D] = (T)0.f;
+      if (on1) y0[(long)t * a.D + 1] = (T)0.f;
     }
+  }
   // the chunk that holds the last token leaves the state (chunks read `state` in scan_join_kernel only)
   if (a.state && len > t0 && len <= tend) {
 #pragma unroll
@@ -418,10 +476,9 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
   }
 }
 
-// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A lane per (channel, state), 8 waves
-// share the chunks: each joins its own run of them, then starts again from the runs before it.
-constexpr int SJ_SEG = 8;
-template <int N>
+// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A lane per (channel, state); where there
+// are many chunks 16 waves share them: each joins its own run, then starts again from the runs before it.
+template <int N, int SJ_SEG>
 __global__ __launch_bounds__(64 * SJ_SEG) void scan_join_kernel(ScanStateArgs a) {
   __shared__ float s_p[SJ_SEG][64], s_h[SJ_SEG][64];
   const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6, b = blockIdx.y;
@@ -500,17 +557,18 @@ struct ScanSplit {
   int cpl, nch, wpg, cl, chunks;
 };
 // Chunks cost a second pass over the states, so sequences are cut only where whole ones leave most of the chip idle: into chunks of
-// at least 64 tokens until there are about 4 096 waves (4 a SIMD), and only if that makes at least 4 of them.
+// at least 64 tokens until there are about 8 192 waves (8 a SIMD, so that their uneven spread over the CUs does not count: 4 096 took
+// 1.35 times as long at 2 x 262144 x 96), and only if that makes at least 4 chunks.
 // Two channels a quad (half the LDS reads of B and C) once there are enough waves; one where the latency of few waves counts.
 inline ScanSplit scan_split(int B, int L, int D, int G) {
   ScanSplit s;
   const int dg = D / G;
   const long waves2 = (long)B * G * ((dg + 31) / 32);
-  long want = 4096 / waves2;
+  long want = 8192 / waves2;
   const long most = (L + 63) / 64;
   if (want > most) want = most;
   if (want < 4) want = 1;
-  s.cpl = waves2 * want >= 512 ? 2 : 1;
+  s.cpl = waves2 * want >= 4096 ? 2 : 1;
   long cl = (L + want - 1) / want;
   cl = (cl + SC_TT - 1) / SC_TT * SC_TT;
   s.cl = (int)cl;
@@ -527,18 +585,20 @@ inline ScanSplit scan_split(int B, int L, int D, int G) {
 template <class T, int N, int CPL>
 static int scan_prompt_run(const ScanStateArgs& a, hipStream_t s) {
   const dim3 grid(a.G * a.wpg, a.chunks, a.B), block(a.nch * 4 / CPL);
-  const int lds = SC_TT * (3 * a.nch + 2 * N) * 4;
+  const int lds = SC_TT * (3 * a.nch + 2 * N) * 4, lds1 = SC_TT * (2 * a.nch + N) * 4;
   static DynLdsCache c0, c1, c2;
   hipError_t e;
   if (a.chunks == 1) {
     if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 0>, lds, c0)) != hipSuccess) return (int)e;
     NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 0>), grid, block, lds, s, a);
   } else {
-    if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 1>, lds, c1)) != hipSuccess) return (int)e;
+    if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 1>, lds1, c1)) != hipSuccess) return (int)e;
     if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 2>, lds, c2)) != hipSuccess) return (int)e;
-    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), grid, block, lds, s, a);
+    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), grid, block, lds1, s, a);
     NNZ_LAUNCH_CHECK();
-    NNZ_LAUNCH((scan_join_kernel<N>), dim3((unsigned)(((long)a.D * N + 63) / 64), a.B), dim3(64 * SJ_SEG), 0, s, a);
+    const dim3 jg((unsigned)(((long)a.D * N + 63) / 64), a.B);
+    if (a.chunks > 64) NNZ_LAUNCH((scan_join_kernel<N, 16>), jg, dim3(64 * 16), 0, s, a);
+    else NNZ_LAUNCH((scan_join_kernel<N, 1>), jg, dim3(64), 0, s, a);
     NNZ_LAUNCH_CHECK();
     NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 2>), grid, block, lds, s, a);
   }
