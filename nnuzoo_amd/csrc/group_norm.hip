@@ -27,7 +27,7 @@ struct GnArgs {
   float* cc;          // backward: [N][G][2]: <w dz>, <w dz xhat>
   float* dw;          // [C] or null
   float* db;
-  long N, S, xb, xs, rows;  // rows: of one workgroup
+  long N, S, xb, xs;
   int nblk, C, G, q;        // q = C / G
   int act;
   float slope, eps;
@@ -68,30 +68,68 @@ __device__ __forceinline__ GnPlace gn_place(int cw) {
   return p;
 }
 
-// per-channel sums over the workgroup's row threads: v[V] of every thread -> dst[channel], in a fixed order
+// per-channel sums over the workgroup's row threads, of a pair of values: s[V], t[V] of every thread -> dst_s[channel], dst_t[channel],
+// in a fixed order.  stage: [2 * NT * V].  All threads first share out the rows of a channel, then its partial sums are added.
 template <class A, int V, int NT = GN_NT>
-__device__ __forceinline__ void gn_fold_rows(A* stage, A* dst, const A (&v)[V], const GnPlace& p, int cw) {
+__device__ __forceinline__ void gn_fold_rows(A* stage, A* dst_s, A* dst_t, const A (&s)[V], const A (&t)[V], const GnPlace& p,
+                                             int cw) {
+  A* st2 = stage + NT * V;
+  const int ch = cw * V;
   __syncthreads();
   if (p.on) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) stage[threadIdx.x * V + j] = v[j];
+    for (int j = 0; j < V; ++j) {
+      stage[threadIdx.x * V + j] = s[j];
+      st2[threadIdx.x * V + j] = t[j];
+    }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < cw * V; c += NT) {
-    A s = 0;
-    for (int r = 0; r < p.R; ++r) s += stage[r * cw * V + c];
-    dst[c] = s;
+  if (ch > NT) {
+    for (int c = threadIdx.x; c < ch; c += NT) {
+      A u = 0, v = 0;
+      for (int r = 0; r < p.R; ++r) {
+        u += stage[r * ch + c];
+        v += st2[r * ch + c];
+      }
+      if (dst_s) dst_s[c] = u;
+      if (dst_t) dst_t[c] = v;
+    }
+    return;
+  }
+  const int parts = NT / ch, part = threadIdx.x / ch, c = threadIdx.x - part * ch;
+  A u = 0, v = 0;
+  if (part < parts)
+    for (int r = part; r < p.R; r += parts) {
+      u += stage[r * ch + c];
+      v += st2[r * ch + c];
+    }
+  __syncthreads();
+  if (part < parts) {
+    stage[threadIdx.x] = u;
+    st2[threadIdx.x] = v;
+  }
+  __syncthreads();
+  if (part == 0) {
+    const int n = parts < p.R ? parts : p.R;
+    for (int k = 1; k < n; ++k) {
+      u += stage[k * ch + c];
+      v += st2[k * ch + c];
+    }
+    if (dst_s) dst_s[c] = u;
+    if (dst_t) dst_t[c] = v;
   }
 }
 
+// A thread's sums are taken about its own first value of each channel, in fp32, and become sums about 0 in fp64 once its rows are
+// done: sum (x - k)^2 is at most a small multiple of what these rows and k add to the variance, so the rounding of fp32 sums of
+// m terms costs m * 2^-24 of the variance at the very most, whatever mu / sigma is.  (fp64 sums throughout: 72 us instead of
+// GNSTATS_US at 2 x 128^3 x 32 f16.)
 template <class TI, int V>
 __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) double gn_lds_d[];
-  double* stage = gn_lds_d;             // [GN_NT * V]
-  double* sums = gn_lds_d + GN_NT * V;  // [2][C]
-  const long n = blockIdx.x / a.nblk;
-  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
-  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  double* stage = gn_lds_d;                 // [2][GN_NT * V]
+  double* sums = gn_lds_d + 2 * GN_NT * V;  // [2][C]
+  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
   const TI* xn = (const TI*)a.x + n * a.xb;
   const int CV = a.C / V;
   for (int c0 = 0; c0 < CV; c0 += GN_NT) {
@@ -100,22 +138,34 @@ __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
     double s[V], sq[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) s[j] = sq[j] = 0.0;
-    if (p.on) {
-      const TI* xc = xn + (long)(c0 + p.col) * V;
+    const long first = blk * p.R + p.rr, hop = (long)a.nblk * p.R;
+    if (p.on && first < a.S) {
+      const TI* xc = xn + (long)(c0 + p.col) * V + first * a.xs;
+      const long step = hop * a.xs;
+      float k[V], d1[V], d2[V];
+      ld_elems<TI, V>(xc, k);
+#pragma unroll
+      for (int j = 0; j < V; ++j) d1[j] = d2[j] = 0.f;
+      const long cnt = (a.S - first + hop - 1) / hop;
 #pragma unroll 4
-      for (long r = r0 + p.rr; r < r1; r += p.R) {
+      for (long i = 1; i < cnt; ++i) {
         float v[V];
-        ld_elems<TI, V>(xc + r * a.xs, v);
+        ld_elems<TI, V>(xc + i * step, v);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const double d = (double)v[j];
-          s[j] += d;
-          sq[j] = fma(d, d, sq[j]);
+          const float d = v[j] - k[j];
+          d1[j] += d;
+          d2[j] = fmaf(d, d, d2[j]);
         }
       }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double kd = k[j], s1 = d1[j], m = (double)cnt;
+        s[j] = fma(m, kd, s1);
+        sq[j] = fma(kd, fma(m, kd, 2.0 * s1), (double)d2[j]);
+      }
     }
-    gn_fold_rows<double, V>(stage, sums + c0 * V, s, p, cw);
-    gn_fold_rows<double, V>(stage, sums + a.C + c0 * V, sq, p, cw);
+    gn_fold_rows<double, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, sq, p, cw);
   }
   __syncthreads();
   for (int g = threadIdx.x; g < a.G; g += GN_NT) {
@@ -158,28 +208,30 @@ __global__ __launch_bounds__(64) void gn_stats_finish_kernel(GnArgs a) {
   }
 }
 
-// per-channel constants of a thread's V channels
-template <int V>
+// constants of a thread's V channels, which lie in GV groups of V / GV channels (registers decide how many waves hide the loads)
+template <int V, int GV>
 struct GnChan {
-  float mean[V], rstd[V], w[V], b[V];
-};
-template <int V>
-__device__ __forceinline__ void gn_chan(const GnArgs& a, long n, int c, GnChan<V>& k) {
+  float mean[GV], rstd[GV], w[V], b[V];
+  __device__ __forceinline__ void load(const GnArgs& a, long n, int c) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float* st = a.stats + (n * a.G + (c + j) / a.q) * 2;
-    k.mean[j] = st[0];
-    k.rstd[j] = st[1];
-    k.w[j] = a.w ? a.w[c + j] : 1.f;
-    k.b[j] = a.b ? a.b[c + j] : 0.f;
+    for (int i = 0; i < GV; ++i) {
+      const float* st = a.stats + (n * a.G + (c + i * (V / GV)) / a.q) * 2;
+      mean[i] = st[0];
+      rstd[i] = st[1];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      w[j] = a.w ? a.w[c + j] : 1.f;
+      b[j] = a.b ? a.b[c + j] : 0.f;
+    }
   }
-}
+  __device__ __forceinline__ float xhat(int j, float v) const { return (v - mean[j / (V / GV)]) * rstd[j / (V / GV)]; }
+  __device__ __forceinline__ float z(int j, float xh) const { return fmaf(xh, w[j], b[j]); }
+};
 
-template <class TI, class TO, int V>
+template <class TI, class TO, int V, int GV>
 __global__ __launch_bounds__(GN_NT) void gn_apply_kernel(GnArgs a) {
-  const long n = blockIdx.x / a.nblk;
-  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
-  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
   const TI* xn = (const TI*)a.x + n * a.xb;
   TO* yn = (TO*)a.out + n * a.S * a.C;
   const int CV = a.C / V;
@@ -188,28 +240,26 @@ __global__ __launch_bounds__(GN_NT) void gn_apply_kernel(GnArgs a) {
     const GnPlace p = gn_place(cw);
     if (!p.on) continue;
     const int c = (c0 + p.col) * V;
-    GnChan<V> k;
-    gn_chan<V>(a, n, c, k);
+    GnChan<V, GV> k;
+    k.load(a, n, c);
 #pragma unroll 2
-    for (long r = r0 + p.rr; r < r1; r += p.R) {
+    for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
       float v[V];
       ld_elems<TI, V>(xn + r * a.xs + c, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = gn_act(fmaf((v[j] - k.mean[j]) * k.rstd[j], k.w[j], k.b[j]), a.act, a.slope);
+      for (int j = 0; j < V; ++j) v[j] = gn_act(k.z(j, k.xhat(j, v[j])), a.act, a.slope);
       st_elems<TO, V>(yn + r * a.C + c, v);
     }
   }
 }
 
 // backward sums: per channel sum dz and sum dz xhat of the workgroup's rows, and their weighted sums per group
-template <class TI, class TO, int V>
+template <class TI, class TO, int V, int GV>
 __global__ __launch_bounds__(GN_NT) void gn_bwd_reduce_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) float gn_lds_f[];
-  float* stage = gn_lds_f;             // [GN_NT * V]
-  float* sums = gn_lds_f + GN_NT * V;  // [2][C]
-  const long n = blockIdx.x / a.nblk;
-  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
-  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  float* stage = gn_lds_f;                 // [2][GN_NT * V]
+  float* sums = gn_lds_f + 2 * GN_NT * V;  // [2][C]
+  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
   const TI* xn = (const TI*)a.x + n * a.xb;
   const TO* gn = (const TO*)a.dy + n * a.S * a.C;
   const int CV = a.C / V;
@@ -221,24 +271,23 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_reduce_kernel(GnArgs a) {
     for (int j = 0; j < V; ++j) s[j] = t[j] = 0.f;
     if (p.on) {
       const int c = (c0 + p.col) * V;
-      GnChan<V> k;
-      gn_chan<V>(a, n, c, k);
+      GnChan<V, GV> k;
+      k.load(a, n, c);
 #pragma unroll 2
-      for (long r = r0 + p.rr; r < r1; r += p.R) {
+      for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
         float v[V], g[V];
         ld_elems<TI, V>(xn + r * a.xs + c, v);
         ld_elems<TO, V>(gn + r * a.C + c, g);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float xh = (v[j] - k.mean[j]) * k.rstd[j];
-          const float dz = gn_dact(fmaf(xh, k.w[j], k.b[j]), g[j], a.act, a.slope);
+          const float xh = k.xhat(j, v[j]);
+          const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
           s[j] += dz;
           t[j] = fmaf(dz, xh, t[j]);
         }
       }
     }
-    gn_fold_rows<float, V>(stage, sums + c0 * V, s, p, cw);
-    gn_fold_rows<float, V>(stage, sums + a.C + c0 * V, t, p, cw);
+    gn_fold_rows<float, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, t, p, cw);
   }
   __syncthreads();
   float* cp = a.cpart + (long)blockIdx.x * a.C * 2;
@@ -305,11 +354,9 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_finish_kernel(GnArgs a, long pai
   }
 }
 
-template <class TI, class TO, int V>
+template <class TI, class TO, int V, int GV>
 __global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
-  const long n = blockIdx.x / a.nblk;
-  const long r0 = (blockIdx.x - n * a.nblk) * a.rows;
-  const long r1 = r0 + a.rows < a.S ? r0 + a.rows : a.S;
+  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
   const TI* xn = (const TI*)a.x + n * a.xb;
   const TO* gn = (const TO*)a.dy + n * a.S * a.C;
   TI* on = (TI*)a.out + n * a.S * a.C;
@@ -319,25 +366,26 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
     const GnPlace p = gn_place(cw);
     if (!p.on) continue;
     const int c = (c0 + p.col) * V;
-    GnChan<V> k;
-    gn_chan<V>(a, n, c, k);
-    float m1[V], m2[V];
+    GnChan<V, GV> k;
+    k.load(a, n, c);
+    float m1[GV], m2[GV];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float* cc = a.cc + (n * a.G + (c + j) / a.q) * 2;
-      m1[j] = cc[0];
-      m2[j] = cc[1];
+    for (int i = 0; i < GV; ++i) {
+      const float* cc = a.cc + (n * a.G + (c + i * (V / GV)) / a.q) * 2;
+      m1[i] = cc[0];
+      m2[i] = cc[1];
     }
 #pragma unroll 2
-    for (long r = r0 + p.rr; r < r1; r += p.R) {
+    for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
       float v[V], g[V];
       ld_elems<TI, V>(xn + r * a.xs + c, v);
       ld_elems<TO, V>(gn + r * a.C + c, g);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float xh = (v[j] - k.mean[j]) * k.rstd[j];
-        const float dz = gn_dact(fmaf(xh, k.w[j], k.b[j]), g[j], a.act, a.slope);
-        v[j] = k.rstd[j] * (k.w[j] * dz - m1[j] - xh * m2[j]);
+        constexpr int Q = V / GV;
+        const float xh = k.xhat(j, v[j]);
+        const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
+        v[j] = k.rstd[j / Q] * (k.w[j] * dz - m1[j / Q] - xh * m2[j / Q]);
       }
       st_elems<TI, V>(on + r * a.C + c, v);
     }
@@ -421,7 +469,7 @@ __global__ __launch_bounds__(GN_SNT) void gn_small_fwd_kernel(GnArgs a) {
 template <class TI, class TO, int V>
 __global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a) {
   __shared__ double red[2 * GN_SNT / 64];
-  __shared__ float stage[GN_SNT * V];
+  __shared__ float stage[2 * GN_SNT * V];
   const int g = blockIdx.x, cw = a.q / V;
   const GnPlace p = gn_place<GN_SNT>(cw);
   const int c = g * a.q + p.col * V;
@@ -475,22 +523,22 @@ __global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a) {
       }
     }
   }
-  if (a.db) gn_fold_rows<float, V, GN_SNT>(stage, a.db + g * a.q, sb, p, cw);
-  if (a.dw) gn_fold_rows<float, V, GN_SNT>(stage, a.dw + g * a.q, sw, p, cw);
+  gn_fold_rows<float, V, GN_SNT>(stage, a.db ? a.db + g * a.q : nullptr, a.dw ? a.dw + g * a.q : nullptr, sb, sw, p, cw);
 }
 
-constexpr int GN_MAX_C = 4096;    // 2 x C fp64 sums and 256 x V fp64 staging fit LDS
-constexpr long GN_TARGET = 1024;  // workgroups of a launch
-// rows of a workgroup: enough workgroups to fill the chip, at least 8 passes over the rows that its threads cover at once
-inline void gn_split(GnArgs& a, int V) {
+constexpr int GN_MAX_C = 4096;    // C and 256 x V fp64 pairs fit LDS
+constexpr long GN_TARGET = 1024;  // workgroups of a launch that sums
+constexpr long GN_TARGET_APPLY = 2048;  // of one that writes (1 024: 120 us instead of 95 for the forward at 2 x 128^3 x 32 f16)
+// Workgroups of a sample: enough to fill the chip, with at least 8 passes over the rows that their threads cover at once.  The rows
+// are dealt out in turn, so that the chip reads one moving window: runs of rows a workgroup lie a power of two apart on the usual
+// sizes, and their streams then meet in the same memory channels (CONTIG_US).
+inline void gn_split(GnArgs& a, int V, long target) {
   const int CV = a.C / V;
   const long R = CV >= GN_NT ? 1 : GN_NT / CV;
-  long per = (GN_TARGET + a.N - 1) / a.N;
+  long per = (target + a.N - 1) / a.N;
   const long most = (a.S + 8 * R - 1) / (8 * R);
   if (per > most) per = most;
-  if (per < 1) per = 1;
-  a.rows = (a.S + per - 1) / per;
-  a.nblk = (int)((a.S + a.rows - 1) / a.rows);
+  a.nblk = (int)(per < 1 ? 1 : per);
 }
 // elements of a workgroup up to which the one-launch kernels are taken, samples that the backward may walk in turn
 constexpr long GN_SMALL_FWD = 16384, GN_SMALL_BWD = 32768, GN_SMALL_N = 8;
@@ -515,51 +563,55 @@ inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
   return w;
 }
 
-template <class TI, class TO, int V>
-static int gn_run_fwd(GnArgs a, hipStream_t s) {
-  if (gn_small(a.N, a.S, a.q, false)) {
-    const dim3 small((unsigned)(a.N * a.G));
-    if (a.q % V == 0) NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, V>), small, dim3(GN_SNT), 0, s, a);
-    else NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, 1>), small, dim3(GN_SNT), 0, s, a);
-    NNZ_LAUNCH_CHECK();
-    return NNZ_OK;
-  }
+template <class TI, class TO, int V, int GV>
+static int gn_large_fwd(GnArgs a, hipStream_t s) {
   static DynLdsCache cache;
-  gn_split(a, V);
-  const int lds = (GN_NT * V + 2 * a.C) * 8;
+  gn_split(a, V, GN_TARGET);
+  const int lds = (GN_NT * V + a.C) * 2 * 8;
   hipError_t e = ensure_dyn_lds((const void*)gn_stats_kernel<TI, V>, lds, cache);
   if (e != hipSuccess) return (int)e;
-  const dim3 grid((unsigned)(a.N * a.nblk));
-  NNZ_LAUNCH((gn_stats_kernel<TI, V>), grid, dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH((gn_stats_kernel<TI, V>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), lds, s, a);
   NNZ_LAUNCH_CHECK();
   NNZ_LAUNCH(gn_stats_finish_kernel, dim3((unsigned)(a.N * a.G)), dim3(64), 0, s, a);
   NNZ_LAUNCH_CHECK();
-  NNZ_LAUNCH((gn_apply_kernel<TI, TO, V>), grid, dim3(GN_NT), 0, s, a);
+  gn_split(a, V, GN_TARGET_APPLY);
+  NNZ_LAUNCH((gn_apply_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), 0, s, a);
   NNZ_LAUNCH_CHECK();
   return NNZ_OK;
 }
-template <class TI, class TO, int V>
-static int gn_run_bwd(GnArgs a, hipStream_t s) {
-  if (gn_small(a.N, a.S, a.q, true)) {
-    if (a.q % V == 0) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, V>), dim3(a.G), dim3(GN_SNT), 0, s, a);
-    else NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, 1>), dim3(a.G), dim3(GN_SNT), 0, s, a);
-    NNZ_LAUNCH_CHECK();
-    return NNZ_OK;
-  }
+template <class TI, class TO, int V, int GV>
+static int gn_large_bwd(GnArgs a, hipStream_t s) {
   static DynLdsCache cache;
-  gn_split(a, V);
-  const int lds = (GN_NT * V + 2 * a.C) * 4;
-  hipError_t e = ensure_dyn_lds((const void*)gn_bwd_reduce_kernel<TI, TO, V>, lds, cache);
+  gn_split(a, V, GN_TARGET);
+  const int lds = (GN_NT * V + a.C) * 2 * 4;
+  hipError_t e = ensure_dyn_lds((const void*)gn_bwd_reduce_kernel<TI, TO, V, GV>, lds, cache);
   if (e != hipSuccess) return (int)e;
-  const dim3 grid((unsigned)(a.N * a.nblk));
-  NNZ_LAUNCH((gn_bwd_reduce_kernel<TI, TO, V>), grid, dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH((gn_bwd_reduce_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), lds, s, a);
   NNZ_LAUNCH_CHECK();
   const long pair_wgs = (a.N * a.G + 3) / 4;
   NNZ_LAUNCH(gn_bwd_finish_kernel, dim3((unsigned)(pair_wgs + (a.C + GN_FC - 1) / GN_FC)), dim3(GN_NT), 0, s, a, pair_wgs);
   NNZ_LAUNCH_CHECK();
-  NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V>), grid, dim3(GN_NT), 0, s, a);
+  gn_split(a, V, GN_TARGET_APPLY);
+  NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), 0, s, a);
   NNZ_LAUNCH_CHECK();
   return NNZ_OK;
+}
+template <class TI, class TO, int V>
+static int gn_run(const GnArgs& a, bool bwd, hipStream_t s) {
+  if (gn_small(a.N, a.S, a.q, bwd)) {
+    const dim3 grid((unsigned)(bwd ? a.G : a.N * a.G));
+    if (bwd && a.q % V == 0) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, V>), grid, dim3(GN_SNT), 0, s, a);
+    else if (bwd) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, 1>), grid, dim3(GN_SNT), 0, s, a);
+    else if (a.q % V == 0) NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, V>), grid, dim3(GN_SNT), 0, s, a);
+    else NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, 1>), grid, dim3(GN_SNT), 0, s, a);
+    NNZ_LAUNCH_CHECK();
+    return NNZ_OK;
+  }
+  // a vector's channels in one group, in two, or anyhow
+  if (a.q % V == 0) return bwd ? gn_large_bwd<TI, TO, V, 1>(a, s) : gn_large_fwd<TI, TO, V, 1>(a, s);
+  if constexpr (V > 2)
+    if (2 * a.q == V) return bwd ? gn_large_bwd<TI, TO, V, 2>(a, s) : gn_large_fwd<TI, TO, V, 2>(a, s);
+  return bwd ? gn_large_bwd<TI, TO, V, V>(a, s) : gn_large_fwd<TI, TO, V, V>(a, s);
 }
 
 // V: the widest of 16 bytes, 4 elements and 1 that the channel count, the strides and the pointers allow
@@ -571,9 +623,9 @@ static int gn_dispatch(const GnArgs& a, bool bwd, hipStream_t s) {
     return a.C % v == 0 && a.xs % v == 0 && a.xb % v == 0 && ((uintptr_t)a.x & ai) == 0 && out == 0 && dy == 0;
   };
   constexpr int FULL = 16 / (int)sizeof(TI);
-  if (fits(FULL)) return bwd ? gn_run_bwd<TI, TO, FULL>(a, s) : gn_run_fwd<TI, TO, FULL>(a, s);
-  if (FULL != 4 && fits(4)) return bwd ? gn_run_bwd<TI, TO, 4>(a, s) : gn_run_fwd<TI, TO, 4>(a, s);
-  return bwd ? gn_run_bwd<TI, TO, 1>(a, s) : gn_run_fwd<TI, TO, 1>(a, s);
+  if (fits(FULL)) return gn_run<TI, TO, FULL>(a, bwd, s);
+  if (FULL != 4 && fits(4)) return gn_run<TI, TO, 4>(a, bwd, s);
+  return gn_run<TI, TO, 1>(a, bwd, s);
 }
 static int gn_go(const GnArgs& a, int ti, int to, bool bwd, hipStream_t s) {
   if (ti == ELEM_F32 && to == ELEM_F32) return gn_dispatch<float, float>(a, bwd, s);
