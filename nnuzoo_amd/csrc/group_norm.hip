@@ -122,8 +122,8 @@ __device__ __forceinline__ void gn_fold_rows(A* stage, A* dst_s, A* dst_t, const
 
 // A thread's sums are taken about its own first value of each channel, in fp32, and become sums about 0 in fp64 once its rows are
 // done: sum (x - k)^2 is at most a small multiple of what these rows and k add to the variance, so the rounding of fp32 sums of
-// m terms costs m * 2^-24 of the variance at the very most, whatever mu / sigma is.  (fp64 sums throughout: 72 us instead of
-// GNSTATS_US at 2 x 128^3 x 32 f16.)
+// m terms costs m * 2^-24 of the variance at the very most, whatever mu / sigma is.  (At 2 x 128^3 x 32 f16: 58 us, 4.6 TB/s;
+// plain reads reach 6.4 here.)
 template <class TI, int V>
 __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) double gn_lds_d[];
@@ -147,7 +147,7 @@ __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) d1[j] = d2[j] = 0.f;
       const long cnt = (a.S - first + hop - 1) / hop;
-#pragma unroll 4
+#pragma unroll 2
       for (long i = 1; i < cnt; ++i) {
         float v[V];
         ld_elems<TI, V>(xc + i * step, v);
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(GN_NT) void gn_apply_kernel(GnArgs a) {
     const int c = (c0 + p.col) * V;
     GnChan<V, GV> k;
     k.load(a, n, c);
-#pragma unroll 2
+#pragma unroll 1
     for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
       float v[V];
       ld_elems<TI, V>(xn + r * a.xs + c, v);
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
       m1[i] = cc[0];
       m2[i] = cc[1];
     }
-#pragma unroll 2
+#pragma unroll 1
     for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
       float v[V], g[V];
       ld_elems<TI, V>(xn + r * a.xs + c, v);
@@ -528,10 +528,11 @@ __global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a) {
 
 constexpr int GN_MAX_C = 4096;    // C and 256 x V fp64 pairs fit LDS
 constexpr long GN_TARGET = 1024;  // workgroups of a launch that sums
-constexpr long GN_TARGET_APPLY = 2048;  // of one that writes (1 024: 120 us instead of 95 for the forward at 2 x 128^3 x 32 f16)
+constexpr long GN_TARGET_APPLY = 4096;  // of one that writes (1 024: 119 us instead of 89 for the forward at 2 x 128^3 x 32 f16)
 // Workgroups of a sample: enough to fill the chip, with at least 8 passes over the rows that their threads cover at once.  The rows
 // are dealt out in turn, so that the chip reads one moving window: runs of rows a workgroup lie a power of two apart on the usual
-// sizes, and their streams then meet in the same memory channels (CONTIG_US).
+// sizes, and their streams then meet in the same memory channels (stats / apply / reduce at 2 x 128^3 x 32 f16: 63 / 92 / 140 us that way, 58 /
+// 89 / 130 in turn).
 inline void gn_split(GnArgs& a, int V, long target) {
   const int CV = a.C / V;
   const long R = CV >= GN_NT ? 1 : GN_NT / CV;

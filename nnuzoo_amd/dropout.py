@@ -19,10 +19,9 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from ._lib import HipCallError, ptr
-from .launch import ELEM, launch, need_device, need_elem
+from .launch import ELEM, first_order, launch, need_device, need_elem
 
 
 def dropout_state(seed: int, device, step: int = 0) -> torch.Tensor:
@@ -52,18 +51,25 @@ class _DropoutFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        used, = ctx.saved_tensors
-        threshold, scale, site, xt, rt = ctx.cfg
-        dx = None
-        if ctx.needs_input_grad[0]:
-            g = dy.contiguous()
-            dx = torch.empty(g.shape, dtype=xt, device=g.device)
-            if dx.numel():
-                launch("nnz_dropout_backward", g.device, g.data_ptr(), ELEM[g.dtype], dx.data_ptr(), ELEM[xt], dx.numel(), threshold,
-                       scale, site, used.data_ptr())
-        return dx, dy.to(rt) if rt is not None and ctx.needs_input_grad[1] else None, None, None, None, None
+        if not torch.is_grad_enabled():
+            return _backward(ctx, dy)
+        with torch.no_grad():
+            grads = _backward(ctx, dy)
+        return first_order("dropout", grads, (dy,))
+
+
+def _backward(ctx, dy):
+    used, = ctx.saved_tensors
+    threshold, scale, site, xt, rt = ctx.cfg
+    dx = None
+    if ctx.needs_input_grad[0]:
+        g = dy.contiguous()
+        dx = torch.empty(g.shape, dtype=xt, device=g.device)
+        if dx.numel():
+            launch("nnz_dropout_backward", g.device, g.data_ptr(), ELEM[g.dtype], dx.data_ptr(), ELEM[xt], dx.numel(), threshold,
+                   scale, site, used.data_ptr())
+    return dx, dy.to(rt) if rt is not None and ctx.needs_input_grad[1] else None, None, None, None, None
 
 
 def _check_p(name, p):

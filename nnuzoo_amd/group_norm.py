@@ -15,10 +15,9 @@ from typing import Optional
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from ._lib import load, ptr
-from .launch import ELEM, launch, need_device, need_elem
+from .launch import ELEM, first_order, launch, need_device, need_elem
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
 MAX_CHANNELS = 4096     # csrc/group_norm.hip GN_MAX_C
@@ -61,25 +60,32 @@ class _GroupNormActFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        xb, xs, groups, act, slope = ctx.cfg
-        dev, N, C = x.device, x.shape[0], x.shape[-1]
-        need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-        make = torch.empty if stats is not None else torch.zeros
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dw = make(C, dtype=torch.float32, device=dev) if need_w else None
-        db = make(C, dtype=torch.float32, device=dev) if need_b else None
-        if stats is not None:
-            dy = dy.contiguous()
-            S = x.numel() // (N * C)
-            ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-            launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
-                   ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C,
-                   groups, act, slope)
-        return dx, dw, db, None, None, None, None, None
+        if not torch.is_grad_enabled():
+            return _backward(ctx, dy)
+        with torch.no_grad():
+            grads = _backward(ctx, dy)
+        return first_order("group_norm_act", grads, (dy, *ctx.saved_tensors[:3]))
+
+
+def _backward(ctx, dy):
+    x, weight, bias, stats = ctx.saved_tensors
+    xb, xs, groups, act, slope = ctx.cfg
+    dev, N, C = x.device, x.shape[0], x.shape[-1]
+    need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
+    make = torch.empty if stats is not None else torch.zeros
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dw = make(C, dtype=torch.float32, device=dev) if need_w else None
+    db = make(C, dtype=torch.float32, device=dev) if need_b else None
+    if stats is not None:
+        dy = dy.contiguous()
+        S = x.numel() // (N * C)
+        ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+        launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
+               ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C,
+               groups, act, slope)
+    return dx, dw, db, None, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,

@@ -44,3 +44,20 @@ def launch(name: str, device: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(device.index))
     if rc:
         check(rc, name)
+
+
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, out, *sources):
+        ctx.name = name
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def first_order(name: str, grads, sources):
+    """`grads` of a backward that is itself being recorded (create_graph=True): usable as values, an error once something is
+    differentiated through them - also where only the saved `sources`, not the incoming gradient, require one"""
+    return tuple(g if g is None else _Once.apply(name, g, *(s for s in sources if s is not None)) for g in grads)

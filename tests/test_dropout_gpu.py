@@ -238,6 +238,10 @@ def test_refusals(hip_lib):
         dropout(x, 0.5, state.cpu())
     with pytest.raises(NotImplementedError, match="float32"):
         dropout(x.double(), 0.5, state)
+    xr, dy = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(dropout(xr, 0.5, state), xr, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        dx.sum().backward()
 
 
 def test_refuses_cpu_tensors_and_bad_calls_without_a_gpu():

@@ -268,10 +268,14 @@ def test_refusals(hip_lib):
         group_norm_act(x, 2, w.cpu(), b)
     with pytest.raises(NotImplementedError, match="activation"):
         GroupNormAct(2, 8, activation="mish")
-    xr = x.clone().requires_grad_(True)
-    dx, = torch.autograd.grad(group_norm_act(xr, 2, w, b).sum(), xr, create_graph=True)
-    with pytest.raises(RuntimeError):
-        dx.sum().backward()
+    # a gradient of the gradient: the first one is a value, the second an error, whichever of its sources asks for it
+    xr, wr = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(group_norm_act(xr, 2, w, b), xr, torch.ones_like(x), create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (dx.square().sum() + xr.sum()).backward()
+    dx, = torch.autograd.grad(group_norm_act(xr, 2, wr, b), xr, torch.ones_like(x), create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(dx.sum(), wr)
     assert issubclass(HipCallError, RuntimeError)
 
 
