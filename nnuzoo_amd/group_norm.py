@@ -104,9 +104,12 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     if C > MAX_CHANNELS:
         raise NotImplementedError(f"group_norm_act: at most {MAX_CHANNELS} channels, got {C}")
     for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and tuple(p.shape) != (C,):
+        if p is not None and p.shape != (C,):
             raise ValueError(f"group_norm_act: `{name}` has shape {tuple(p.shape)}, expected ({C},)")
-    weight, bias = (p if p is None else p.float().contiguous() for p in (weight, bias))
+    if weight is not None:
+        weight = weight.float().contiguous()
+    if bias is not None:
+        bias = bias.float().contiguous()
     out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
     return _GroupNormActFn.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation], float(negative_slope),
                                  out_dtype)

@@ -13,14 +13,14 @@ def need_device(name: str, *tensors) -> torch.device:
     """the one device of all tensors (None is skipped); CPU tensors and mixed devices are refused"""
     dev = None
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"nnuzoo_amd.{name} runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise HipCallError(f"{name}: tensors on {dev} and {t.device}")
+        if t is not None:
+            d = t.device
+            if dev is None:
+                dev = d
+            if d != dev or d.type != "cuda":
+                if d.type != "cuda" or dev.type != "cuda":
+                    raise RuntimeError(f"nnuzoo_amd.{name} runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+                raise HipCallError(f"{name}: tensors on {dev} and {d}")
     return dev
 
 

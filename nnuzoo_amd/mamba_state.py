@@ -35,33 +35,38 @@ STATE_WIDTHS = (4, 8, 16, 32)
 
 
 def _no_grad(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() (training goes through "
-                           "nnuzoo_amd.mamba_block.causal_conv1d_fn and nnuzoo_amd.selective_scan.selective_scan_fn)")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward: call it under torch.no_grad() (training goes through "
+                                   "nnuzoo_amd.mamba_block.causal_conv1d_fn and nnuzoo_amd.selective_scan.selective_scan_fn)")
 
 
 def _shape(name, arg, t, shape):
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: `{arg}` has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _inner(t):
     """t with adjacent elements along the last axis"""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _param(t):
-    return None if t is None else t.detach().float().contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
 
 
 def _own_memory(name, arg, t):
     """a state is written in place: no two of its elements may share memory"""
+    if t.is_contiguous():
+        return
     need = 1
     for stride, size in sorted((t.stride(d), t.shape[d]) for d in range(t.dim()) if t.shape[d] > 1):
         if stride < need:
             raise ValueError(f"{name}: elements of `{arg}` share memory (shape {tuple(t.shape)}, strides {t.stride()})")
         need = stride * (size - 1) + need
-    return t
 
 
 def _which(name, arg, t, batch, kinds):
@@ -84,6 +89,8 @@ def _conv_checks(name, x, weight, bias, activation, conv_state, rows):
     if weight.dim() == 3 and weight.shape[1] == 1:
         weight = weight.squeeze(1)      # nn.Conv1d's layout
     W = weight.shape[-1]
+    if weight.dim() != 2:
+        raise ValueError(f"{name}: `weight` has shape {tuple(weight.shape)}, expected {(D, 'W')}")
     _shape(name, "weight", weight, (D, W))
     if not 1 <= W <= MAX_WIDTH:
         raise NotImplementedError(f"{name}: kernel widths 1 .. {MAX_WIDTH}, got {W}")
@@ -136,41 +143,47 @@ def causal_conv1d_token(x: torch.Tensor, conv_state: torch.Tensor, weight: torch
 
 
 def _scan_checks(name, x, dt, A, B, C, D, z, dt_bias, state, rows):
-    lead = tuple(x.shape[:-1])
+    """checks and brings into form: (x, dt, B, C, z, A, D, dt_bias, channels, heads, groups, state width)"""
     if x.dim() != rows:
         raise ValueError(f"{name}: x must be {'(B, L, D)' if rows == 3 else '(B, D)'}, got {tuple(x.shape)}")
-    need_elem(name, x=x, dt=dt, B=B, C=C, z=z, A=A, D=D, dt_bias=dt_bias)
+    need_elem(name, x=x, A=A, D=D, dt_bias=dt_bias)
     _no_grad(name, x, dt, A, B, C, D, z, dt_bias, state)
     for arg, t in (("dt", dt), ("B", B), ("C", C), ("z", z)):
-        if t is not None and t.dtype != x.dtype:
+        if t is not None and t.dtype is not x.dtype:
             raise TypeError(f"{name}: x is {x.dtype}, `{arg}` is {t.dtype}: activations share one type")
-    d, h = x.shape[-1], dt.shape[-1]
-    _shape(name, "dt", dt, lead + (h,))
+    *lead, d = x.shape
+    h = dt.shape[-1]
+    _shape(name, "dt", dt, (*lead, h))
     if z is not None:
         _shape(name, "z", z, x.shape)
-    B, C = (t.unsqueeze(-2) if t.dim() == rows else t for t in (B, C))
+    if B.dim() == rows:
+        B = B.unsqueeze(-2)
+    if C.dim() == rows:
+        C = C.unsqueeze(-2)
     if B.dim() != rows + 1:
         raise ValueError(f"{name}: `B` has {B.dim()} dimensions, expected {rows} or {rows + 1}")
     g, n = B.shape[-2:]
-    _shape(name, "B", B, lead + (g, n))
-    _shape(name, "C", C, lead + (g, n))
+    _shape(name, "B", B, (*lead, g, n))
+    _shape(name, "C", C, B.shape)
     if n not in STATE_WIDTHS:
         raise NotImplementedError(f"{name}: state widths {STATE_WIDTHS}, got {n}")
     if h < 1 or g < 1 or d % h or h % g:
         raise ValueError(f"{name}: {d} channels, {h} heads, {g} groups: heads divide the channels, groups divide the heads")
-    if tuple(A.shape) not in ((h, n), (h,)):
+    if A.shape != (h, n) and A.shape != (h,):
         raise ValueError(f"{name}: `A` has shape {tuple(A.shape)}, expected {(h, n)} or {(h,)}")
-    for arg, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None:
-            _shape(name, arg, t, (h,))
+    if D is not None:
+        _shape(name, "D", D, (h,))
+    if dt_bias is not None:
+        _shape(name, "dt_bias", dt_bias, (h,))
     if state is not None:
-        if state.dtype != torch.float32:
+        if state.dtype is not torch.float32:
             raise TypeError(f"{name}: `state` must be float32, got {state.dtype}")
-        _shape(name, "state", state, (x.shape[0], d, n))
-        if d and (state.stride(2) != 1 or (d > 1 and state.stride(1) != n)):
-            raise ValueError(f"{name}: `state` is updated in place and must be contiguous within a sequence, strides {state.stride()}")
-        _own_memory(name, "state", state)
-    return tuple(None if t is None else _inner(t) for t in (x, dt, B, C, z)) + tuple(_param(t) for t in (A, D, dt_bias)) + (d, h, g, n)
+        _shape(name, "state", state, (lead[0], d, n))
+        if d and not state.is_contiguous():
+            if state.stride(2) != 1 or (d > 1 and state.stride(1) != n):
+                raise ValueError(f"{name}: `state` is updated in place and must be contiguous within a sequence, strides {state.stride()}")
+            _own_memory(name, "state", state)
+    return _inner(x), _inner(dt), _inner(B), _inner(C), _inner(z), _param(A), _param(D), _param(dt_bias), d, h, g, n
 
 
 _Long7, _Long12 = ctypes.c_long * 7, ctypes.c_long * 12
@@ -189,7 +202,8 @@ def selective_scan_prompt(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     lengths = _which(name, "lengths", lengths, batch, (torch.int32, torch.int64))
     y = torch.empty((batch, L, d), dtype=x.dtype, device=dev)
     if y.numel():
-        strides = _Long12(*x.stride()[:2], *dt.stride()[:2], *B.stride()[:3], *C.stride()[:3], *(z.stride()[:2] if z is not None else (0, 0)))
+        strides = _Long12(*x.stride()[:2], *dt.stride()[:2], *B.stride()[:3], *C.stride()[:3],
+                          *(z.stride()[:2] if z is not None else (0, 0)))
         ws_bytes = load().nnz_selective_scan_prompt_workspace_bytes(batch, L, d, h, g, n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_selective_scan_prompt", dev, x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(z), ELEM[x.dtype],
