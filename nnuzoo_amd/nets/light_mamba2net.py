@@ -9,7 +9,8 @@ axis order ('h w' / 'w h' in 2-D; 'd h w' / 'd w h' / 'w h d' in 3-D, cycling wi
 pooling by the per-axis scales of get_scales(min_size=4), up-sampling a 1x1 conv + (bi/tri)linear interpolation.
 
 The mixer is nnuzoo_amd.nets.mamba2.Mamba2 (the SSD recurrence on the HIP chunk-scan / causal-conv1d / gate kernels);
-LayerNorm is the HIP layer_norm kernel; everything else is small-channel fp32 convolution / GroupNorm / InstanceNorm glue.
+LayerNorm is the HIP layer_norm kernel; a GroupNorm + activation that follows a mixer (token-major memory) is the HIP group norm
+kernel; everything else is small-channel fp32 convolution / GroupNorm / InstanceNorm glue.
 Attribute names follow the reference class line by line (same state_dict keys).  monai helpers restated here:
 get_upsample_layer(nontrainable) = nn.Upsample(linear, align_corners=False); get_norm_layer(("GROUP", {num_groups: 8}))
 = nn.GroupNorm(8, C); get_act_layer(("RELU", {inplace})) = nn.ReLU (PARITY UNPINNED for those, as nets/monai_blocks.py).
@@ -23,6 +24,7 @@ import numpy as np
 import torch
 from torch import nn
 
+from ..group_norm import norm_act
 from ..layer_norm import LayerNorm
 from ..token_linear import TokenLinear
 from ..utilities.network_initialization import InitWeights_He
@@ -145,9 +147,9 @@ class ResUpBlock(nn.Module):
 
     def forward(self, x):
         identity = x
-        x = self.act(self.norm1(x))
+        x = norm_act(self.norm1, self.act, x)
         x = self.conv(x) + self.skip_scale * identity
-        return self.act(self.norm2(x))
+        return norm_act(self.norm2, self.act, x)
 
 
 _AXES = {2: "hw", 3: "dhw"}
@@ -181,8 +183,8 @@ class ResMambaBlock(nn.Module):
     def forward(self, x):
         x = self.gsc(x)
         identity = x
-        x = self.nd_mamba_order(self.order, self.act(self.norm1(x)), self.mamba1)
-        x = self.nd_mamba_order(self.order, self.act(self.norm2(x)), self.mamba2)
+        x = self.nd_mamba_order(self.order, norm_act(self.norm1, self.act, x), self.mamba1)
+        x = self.nd_mamba_order(self.order, norm_act(self.norm2, self.act, x), self.mamba2)
         return x + identity
 
 

@@ -18,6 +18,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from ..group_norm import norm_act
 from ..layer_norm import LayerNorm
 from ..token_linear import TokenLinear
 from ..utilities.network_initialization import InitWeights_He
@@ -68,8 +69,8 @@ class ResMambaBlock(nn.Module):
     def forward(self, x):
         x = self.gsc(x)
         identity = x
-        x = self.conv1(self.act(self.norm1(x)))
-        x = self.conv2(self.act(self.norm2(x)))
+        x = self.conv1(norm_act(self.norm1, self.act, x))
+        x = self.conv2(norm_act(self.norm2, self.act, x))
         return x + identity
 
 

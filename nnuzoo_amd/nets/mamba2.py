@@ -21,6 +21,9 @@ MI355X mapping: the SSD recurrence is the selective scan with a per-head scalar 
 csrc/selective_scan.hip with A[(h, p), n] = A[h], delta[(h, p)] = dt[h], D[(h, p)] = D[h] and one B/C group - so the
 block runs on the existing chunk-scan / causal-conv1d / gate kernels; the head -> channel broadcasts are views whose
 gradients autograd sums back per head.  No CPU path: the kernels raise on CPU tensors.
+
+Decoding (`inference_params`, `prompt`, `step`, `allocate_inference_cache`) runs token-major on the state-carrying operators of
+nnuzoo_amd.mamba_state, which take heads as they are; caches: (B, conv_dim, d_conv) and fp32 (B, nheads, headdim, d_state).
 """
 from __future__ import annotations
 
@@ -30,9 +33,11 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .. import mamba_state
 from ..mamba_block import causal_conv1d_fn, silu_gate
 from ..selective_scan import selective_scan_fn
 from ..token_linear import TokenLinear
+from .mamba_simple import decode
 
 
 class RMSNormGated(nn.Module):
@@ -85,10 +90,12 @@ class Mamba2(nn.Module):
 
     def forward(self, u: torch.Tensor, seq_idx=None, inference_params=None) -> torch.Tensor:
         """u (B, L, d_model) -> (B, L, d_model)"""
-        if inference_params is not None or seq_idx is not None:
-            raise NotImplementedError("nnuzoo_amd.Mamba2: step-wise decoding / packed sequences are outside the hot path")
+        if seq_idx is not None:
+            raise NotImplementedError("nnuzoo_amd.Mamba2: packed sequences are outside the hot path")
         if not u.is_cuda:
             raise RuntimeError("nnuzoo_amd.Mamba2 runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+        if inference_params is not None:
+            return decode(self, u, inference_params)
         Bt, L, _ = u.shape
         ds, n = self.d_ssm, self.d_state
         # in_proj produced directly in the channel-major (B, C, L) layout the conv / scan kernels read
@@ -105,7 +112,38 @@ class Mamba2(nn.Module):
         y = self.norm(y, z.contiguous())
         return F.linear(y.transpose(1, 2), self.out_proj.weight, self.out_proj.bias)
 
-    def step(self, *a, **k):
-        raise NotImplementedError("nnuzoo_amd.Mamba2: step-wise decoding is outside the segmentation hot path")
+    # ---- decoding ------------------------------------------------------------------------------------------------------------
+    def _decode(self, u, conv_state, ssm_state, **which):
+        if not u.is_cuda:
+            raise RuntimeError("nnuzoo_amd.Mamba2 runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+        prompt = u.dim() == 3
+        ds, n = self.d_ssm, self.d_state
+        zxbcdt = F.linear(u, self.in_proj.weight, self.in_proj.bias)
+        conv = (self.conv1d.weight, self.conv1d.bias, "silu")
+        xbc = zxbcdt[..., ds:2 * ds + 2 * n]
+        xbc = mamba_state.causal_conv1d_prompt(xbc, *conv, conv_state, **which) if prompt else \
+            mamba_state.causal_conv1d_token(xbc, conv_state, *conv, **which)
+        scan = mamba_state.selective_scan_prompt if prompt else mamba_state.selective_scan_token
+        y = scan(xbc[..., :ds], zxbcdt[..., 2 * ds + 2 * n:], -torch.exp(self.A_log.float()), xbc[..., ds:ds + n], xbc[..., ds + n:],
+                 self.D, z=zxbcdt[..., :ds], dt_bias=self.dt_bias, dt_softplus=True,
+                 state=ssm_state.view(-1, ds, n), **which).float()
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.norm.eps) * self.norm.weight
+        return F.linear(y.to(u.dtype), self.out_proj.weight, self.out_proj.bias)
 
-    allocate_inference_cache = step
+    @torch.no_grad()
+    def prompt(self, u, conv_state, ssm_state, lengths=None):
+        """(B, L, d_model) -> (B, L, d_model); the states are read (zeros: a new sequence) and left behind each sequence's last
+        token.  lengths (B,): tokens of each sequence"""
+        return self._decode(u, conv_state, ssm_state, lengths=lengths)
+
+    @torch.no_grad()
+    def step(self, u, conv_state, ssm_state, active=None):
+        """one token, (B, 1, d_model) -> ((B, 1, d_model), conv_state, ssm_state); the states are updated in place"""
+        if u.dim() != 3 or u.shape[1] != 1:
+            raise ValueError(f"step takes one token a sequence, (B, 1, d_model); got {tuple(u.shape)}")
+        return self._decode(u[:, 0], conv_state, ssm_state, active=active)[:, None], conv_state, ssm_state
+
+    def allocate_inference_cache(self, batch_size, max_seqlen=None, dtype=None, **kwargs):
+        w = self.conv1d.weight
+        return (torch.zeros(batch_size, w.shape[0], self.d_conv, device=w.device, dtype=dtype or w.dtype),
+                torch.zeros(batch_size, self.nheads, self.headdim, self.d_state, device=w.device, dtype=torch.float32))

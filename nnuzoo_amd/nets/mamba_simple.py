@@ -4,8 +4,12 @@ Same constructor, parameters, initialisation sequence and state_dict as the refe
 /root/reference/nnunetv2/nets/seg_mamba/mamba_simple.py:37-190 (used by SegMamba, segmamba.py:74-81; the `mamba_ssm.Mamba`
 the reference binds in lm2net.py:14,70 and mamba_nd2net.py:26 has the bimamba_type="none" subset of it).  forward
 (:190-357) runs on the HIP operators of nnuzoo_amd.mamba_block (causal conv1d + SiLU, selective scan, z gate); the
-projections are library GEMMs.  `use_fast_path` is accepted and ignored: there is one path.  Step-wise decoding
-(`inference_params`, `step`, `allocate_inference_cache`) is not part of the segmentation hot path and raises.
+projections are library GEMMs.  `use_fast_path` is accepted and ignored: there is one path.
+
+Decoding (`inference_params`, `step`, `allocate_inference_cache`: :190-215, 357-411, 413-450) runs token-major on the state-carrying
+operators of nnuzoo_amd.mamba_state, without gradients: `prompt` takes whole prompts (ragged ones by `lengths`) and leaves the states,
+`step` one token a sequence.  The caches have the reference's shapes; the scan state is fp32 whatever the cache's type.  Only the
+causal form exists (bimamba_type "none").
 """
 from __future__ import annotations
 
@@ -15,6 +19,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import mamba_state
 from ..mamba_block import mamba_inner_fn_no_out_proj
 
 
@@ -95,10 +100,10 @@ class Mamba(nn.Module):
 
     def forward(self, hidden_states, inference_params=None):
         """hidden_states (B, L, D) -> (B, L, D)"""
-        if inference_params is not None:
-            raise NotImplementedError("nnuzoo_amd.Mamba: step-wise decoding is outside the segmentation hot path")
         if not hidden_states.is_cuda:
             raise RuntimeError("nnuzoo_amd.Mamba runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+        if inference_params is not None:
+            return decode(self, hidden_states, inference_params)
         batch, seqlen, _ = hidden_states.shape
         # (B, L, D) x W_in^T, produced directly in the (B, 2*d_inner, L) layout the conv / scan read
         xz = (self.in_proj.weight @ hidden_states.reshape(batch * seqlen, -1).t()).view(-1, batch, seqlen).transpose(0, 1)
@@ -116,10 +121,68 @@ class Mamba(nn.Module):
             out = out + out_s.reshape(batch, self.d_inner, seqlen // ns, ns).permute(0, 1, 3, 2).flatten(-2)
         return F.linear(out.transpose(1, 2), self.out_proj.weight, self.out_proj.bias)
 
-    def step(self, *a, **k):
-        raise NotImplementedError("nnuzoo_amd.Mamba: step-wise decoding is outside the segmentation hot path")
+    # ---- decoding ------------------------------------------------------------------------------------------------------------
+    def _decode(self, hidden, conv_state, ssm_state, **which):
+        """(B, L, D) with lengths=..., or (B, D) with active=...: projections, convolution and scan on carried states"""
+        if self.bimamba_type != "none":
+            raise NotImplementedError(f"nnuzoo_amd.Mamba: decoding needs a causal block, this one is bimamba_type={self.bimamba_type!r}")
+        if not hidden.is_cuda:
+            raise RuntimeError("nnuzoo_amd.Mamba runs on MI355X through libnnuzoo_hip.so only (no CPU fallback)")
+        prompt = hidden.dim() == 3
+        di, R, N = self.d_inner, self.dt_rank, self.d_state
+        xz = F.linear(hidden, self.in_proj.weight, self.in_proj.bias)
+        conv = (self.conv1d.weight, self.conv1d.bias, "silu")
+        if prompt:
+            u = mamba_state.causal_conv1d_prompt(xz[..., :di], *conv, conv_state, **which)
+        else:
+            u = mamba_state.causal_conv1d_token(xz[..., :di], conv_state, *conv, **which)
+        dbc = F.linear(u, self.x_proj.weight)
+        dt = F.linear(dbc[..., :R], self.dt_proj.weight)
+        scan = mamba_state.selective_scan_prompt if prompt else mamba_state.selective_scan_token
+        y = scan(u, dt, -torch.exp(self.A_log.float()), dbc[..., R:R + N], dbc[..., R + N:], self.D, z=xz[..., di:],
+                 dt_bias=self.dt_proj.bias, dt_softplus=True, state=ssm_state, **which)
+        return F.linear(y, self.out_proj.weight, self.out_proj.bias)
 
-    allocate_inference_cache = step
+    @torch.no_grad()
+    def prompt(self, hidden_states, conv_state, ssm_state, lengths=None):
+        """(B, L, D) -> (B, L, D); the states are read (zeros: a new sequence) and left behind each sequence's last token.
+        lengths (B,): tokens of each sequence; outputs behind them are those of an all-zero scan output"""
+        return self._decode(hidden_states, conv_state, ssm_state, lengths=lengths)
+
+    @torch.no_grad()
+    def step(self, hidden_states, conv_state, ssm_state, active=None):
+        """one token, (B, 1, D) -> ((B, 1, D), conv_state, ssm_state); the states are updated in place.  active (B,) bool: the
+        sequences that take part"""
+        if hidden_states.dim() != 3 or hidden_states.shape[1] != 1:
+            raise ValueError(f"step takes one token a sequence, (B, 1, D); got {tuple(hidden_states.shape)}")
+        out = self._decode(hidden_states[:, 0], conv_state, ssm_state, active=active)
+        return out[:, None], conv_state, ssm_state
+
+    def allocate_inference_cache(self, batch_size, max_seqlen=None, dtype=None, **kwargs):
+        """(conv_state (B, d_inner, d_conv), ssm_state (B, d_inner, d_state)), zeros; `dtype` is the convolution state's, the
+        activations' type or fp32 (default: the weights' type)"""
+        w = self.conv1d.weight
+        return (torch.zeros(batch_size, self.d_inner, self.d_conv, device=w.device, dtype=dtype or w.dtype),
+                torch.zeros(batch_size, self.d_inner, self.d_state, device=w.device, dtype=torch.float32))
+
+
+def decode(block, hidden_states, inference_params):
+    """forward of a block with `inference_params`: the block's states live in inference_params.key_value_memory_dict[layer_idx]; a
+    prompt (seqlen_offset 0) starts them from zero, with inference_params.lengths_per_sample where it is given, later calls are
+    single tokens"""
+    if block.layer_idx is None:
+        raise ValueError("decoding with inference_params needs the block's layer_idx")
+    memory, batch = inference_params.key_value_memory_dict, hidden_states.shape[0]
+    first = inference_params.seqlen_offset == 0
+    states = memory.get(block.layer_idx)
+    if states is None or (first and states[0].shape[0] != batch):
+        states = memory[block.layer_idx] = block.allocate_inference_cache(batch, getattr(inference_params, "max_seqlen", None))
+    elif first:
+        for t in states:
+            t.zero_()
+    if not first:
+        return block.step(hidden_states, *states)[0]
+    return block.prompt(hidden_states, *states, lengths=getattr(inference_params, "lengths_per_sample", None))
 
 
 class MambaSSM(Mamba):
