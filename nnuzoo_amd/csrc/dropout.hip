@@ -10,7 +10,7 @@
 // Bound by HBM, with integer multiplication close behind: a call is 20 products of 32 x 32 -> 64 bits at a quarter of the vector
 // rate.  One call serves 8 elements because a 16-bit half already decides unless it EQUALS the threshold's upper half; that
 // happens once in 65 536 elements, and only the waves that meet it make the second call - the probability is exact to 2^-32 at
-// half the price of 32-bit draws.
+// half the price of 32-bit draws.  2 x 512^2 x 128 f16: 50 us each way = 5.4 TB/s, what a copy of that size reaches.
 #include "elem_io.hpp"
 
 namespace nnz {

@@ -2,6 +2,8 @@
 //   z = (x - mu[n,g]) * r[n,g] * w[c] + b[c],  y = act(z),  mu / r over the S positions and C / G channels of a group;
 //   dz = dy act'(z),  db = sum dz,  dw = sum dz xhat,  dx = r (w dz - <w dz> - xhat <w dz xhat>)  with <.> the group's mean.
 // Bound by HBM: a group does not fit on chip, so forward reads x twice and writes y, backward reads x and dy twice and writes dx.
+// 2 x 128^3 x 32 f16 (268 MB a tensor), SiLU: sums 59 us (4.5 TB/s), write pass 89 (6.0), backward sums 126 (4.3, the logistic
+// function's share shows), write pass 150 (5.4), finishing launches 5 each.
 //
 // A thread owns V consecutive channels (16 bytes) and walks the rows, a workgroup owns a run of rows of one sample: every access
 // is a run of whole rows whatever the group width, and the group's members meet only after the rows are summed.  Sums of the
@@ -53,6 +55,10 @@ __device__ __forceinline__ float gn_dact(float z, float dy, int act, float slope
   }
 }
 
+// a workgroup takes the parts (samples x a.nblk) of a launch in turn; more parts than a grid may have workgroups are rare
+#define GN_FOR_EACH_PART(a) for (long part = blockIdx.x; part < (a).N * (a).nblk; part += gridDim.x)
+constexpr long GN_MAX_WG = 1L << 22;   // 2^32 threads are too many
+
 // a thread's place: vector columns [c0, c0 + cw) of the row are dealt out over the workgroup, R rows at a time
 struct GnPlace {
   int col, rr, R;
@@ -68,8 +74,9 @@ __device__ __forceinline__ GnPlace gn_place(int cw) {
   return p;
 }
 
-// per-channel sums over the workgroup's row threads, of a pair of values: s[V], t[V] of every thread -> dst_s[channel], dst_t[channel],
-// in a fixed order.  stage: [2 * NT * V].  All threads first share out the rows of a channel, then its partial sums are added.
+// per-channel sums over the workgroup's row threads, of a pair of values: s[V], t[V] of every thread -> dst_s[channel],
+// dst_t[channel], in a fixed order.  stage: [2 * NT * V].  All threads first share out the rows of a channel, then its partial sums
+// are added.
 template <class A, int V, int NT = GN_NT>
 __device__ __forceinline__ void gn_fold_rows(A* stage, A* dst_s, A* dst_t, const A (&s)[V], const A (&t)[V], const GnPlace& p,
                                              int cw) {
@@ -129,54 +136,56 @@ __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) double gn_lds_d[];
   double* stage = gn_lds_d;                 // [2][GN_NT * V]
   double* sums = gn_lds_d + 2 * GN_NT * V;  // [2][C]
-  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
-  const TI* xn = (const TI*)a.x + n * a.xb;
-  const int CV = a.C / V;
-  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
-    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
-    const GnPlace p = gn_place(cw);
-    double s[V], sq[V];
+  GN_FOR_EACH_PART(a) {
+    const long n = part / a.nblk, blk = part - n * a.nblk;
+    const TI* xn = (const TI*)a.x + n * a.xb;
+    const int CV = a.C / V;
+    for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+      const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+      const GnPlace p = gn_place(cw);
+      double s[V], sq[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = sq[j] = 0.0;
-    const long first = blk * p.R + p.rr, hop = (long)a.nblk * p.R;
-    if (p.on && first < a.S) {
-      const TI* xc = xn + (long)(c0 + p.col) * V + first * a.xs;
-      const long step = hop * a.xs;
-      float k[V], d1[V], d2[V];
-      ld_elems<TI, V>(xc, k);
+      for (int j = 0; j < V; ++j) s[j] = sq[j] = 0.0;
+      const long first = blk * p.R + p.rr, hop = (long)a.nblk * p.R;
+      if (p.on && first < a.S) {
+        const TI* xc = xn + (long)(c0 + p.col) * V + first * a.xs;
+        const long step = hop * a.xs;
+        float k[V], d1[V], d2[V];
+        ld_elems<TI, V>(xc, k);
 #pragma unroll
-      for (int j = 0; j < V; ++j) d1[j] = d2[j] = 0.f;
-      const long cnt = (a.S - first + hop - 1) / hop;
+        for (int j = 0; j < V; ++j) d1[j] = d2[j] = 0.f;
+        const long cnt = (a.S - first + hop - 1) / hop;
 #pragma unroll 2
-      for (long i = 1; i < cnt; ++i) {
-        float v[V];
-        ld_elems<TI, V>(xc + i * step, v);
+        for (long i = 1; i < cnt; ++i) {
+          float v[V];
+          ld_elems<TI, V>(xc + i * step, v);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float d = v[j] - k[j];
+            d1[j] += d;
+            d2[j] = fmaf(d, d, d2[j]);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const float d = v[j] - k[j];
-          d1[j] += d;
-          d2[j] = fmaf(d, d, d2[j]);
+          const double kd = k[j], s1 = d1[j], m = (double)cnt;
+          s[j] = fma(m, kd, s1);
+          sq[j] = fma(kd, fma(m, kd, 2.0 * s1), (double)d2[j]);
         }
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double kd = k[j], s1 = d1[j], m = (double)cnt;
-        s[j] = fma(m, kd, s1);
-        sq[j] = fma(kd, fma(m, kd, 2.0 * s1), (double)d2[j]);
+      gn_fold_rows<double, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, sq, p, cw);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < a.G; g += GN_NT) {
+      double s = 0.0, sq = 0.0;
+      for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
+        s += sums[c];
+        sq += sums[a.C + c];
       }
+      double* o = a.gpart + (part * a.G + g) * 2;
+      o[0] = s;
+      o[1] = sq;
     }
-    gn_fold_rows<double, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, sq, p, cw);
-  }
-  __syncthreads();
-  for (int g = threadIdx.x; g < a.G; g += GN_NT) {
-    double s = 0.0, sq = 0.0;
-    for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
-      s += sums[c];
-      sq += sums[a.C + c];
-    }
-    double* o = a.gpart + ((long)blockIdx.x * a.G + g) * 2;
-    o[0] = s;
-    o[1] = sq;
   }
 }
 
@@ -195,16 +204,18 @@ __device__ __forceinline__ void gn_sum_parts(const double* p, int nblk, int G, d
 }
 
 __global__ __launch_bounds__(64) void gn_stats_finish_kernel(GnArgs a) {
-  const long n = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x - n * a.G);
-  double s, sq;
-  gn_sum_parts(a.gpart + (n * a.nblk * a.G + g) * 2, a.nblk, a.G, s, sq);
-  if (threadIdx.x == 0) {
-    const double m = (double)a.S * a.q, mean = s / m;
-    double var = sq / m - mean * mean;
-    if (var < 0.0) var = 0.0;  // NaN stays
-    a.stats[(long)blockIdx.x * 2] = (float)mean;
-    a.stats[(long)blockIdx.x * 2 + 1] = (float)(1.0 / sqrt(var + (double)a.eps));
+  for (long pair = blockIdx.x; pair < a.N * a.G; pair += gridDim.x) {
+    const long n = pair / a.G;
+    const int g = (int)(pair - n * a.G);
+    double s, sq;
+    gn_sum_parts(a.gpart + (n * a.nblk * a.G + g) * 2, a.nblk, a.G, s, sq);
+    if (threadIdx.x == 0) {
+      const double m = (double)a.S * a.q, mean = s / m;
+      double var = sq / m - mean * mean;
+      if (var < 0.0) var = 0.0;  // NaN stays
+      a.stats[pair * 2] = (float)mean;
+      a.stats[pair * 2 + 1] = (float)(1.0 / sqrt(var + (double)a.eps));
+    }
   }
 }
 
@@ -231,24 +242,26 @@ struct GnChan {
 
 template <class TI, class TO, int V, int GV>
 __global__ __launch_bounds__(GN_NT) void gn_apply_kernel(GnArgs a) {
-  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
-  const TI* xn = (const TI*)a.x + n * a.xb;
-  TO* yn = (TO*)a.out + n * a.S * a.C;
-  const int CV = a.C / V;
-  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
-    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
-    const GnPlace p = gn_place(cw);
-    if (!p.on) continue;
-    const int c = (c0 + p.col) * V;
-    GnChan<V, GV> k;
-    k.load(a, n, c);
+  GN_FOR_EACH_PART(a) {
+    const long n = part / a.nblk, blk = part - n * a.nblk;
+    const TI* xn = (const TI*)a.x + n * a.xb;
+    TO* yn = (TO*)a.out + n * a.S * a.C;
+    const int CV = a.C / V;
+    for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+      const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+      const GnPlace p = gn_place(cw);
+      if (!p.on) continue;
+      const int c = (c0 + p.col) * V;
+      GnChan<V, GV> k;
+      k.load(a, n, c);
 #pragma unroll 1
-    for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
-      float v[V];
-      ld_elems<TI, V>(xn + r * a.xs + c, v);
+      for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
+        float v[V];
+        ld_elems<TI, V>(xn + r * a.xs + c, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = gn_act(k.z(j, k.xhat(j, v[j])), a.act, a.slope);
-      st_elems<TO, V>(yn + r * a.C + c, v);
+        for (int j = 0; j < V; ++j) v[j] = gn_act(k.z(j, k.xhat(j, v[j])), a.act, a.slope);
+        st_elems<TO, V>(yn + r * a.C + c, v);
+      }
     }
   }
 }
@@ -259,69 +272,71 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_reduce_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) float gn_lds_f[];
   float* stage = gn_lds_f;                 // [2][GN_NT * V]
   float* sums = gn_lds_f + 2 * GN_NT * V;  // [2][C]
-  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
-  const TI* xn = (const TI*)a.x + n * a.xb;
-  const TO* gn = (const TO*)a.dy + n * a.S * a.C;
-  const int CV = a.C / V;
-  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
-    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
-    const GnPlace p = gn_place(cw);
-    float s[V], t[V];
+  GN_FOR_EACH_PART(a) {
+    const long n = part / a.nblk, blk = part - n * a.nblk;
+    const TI* xn = (const TI*)a.x + n * a.xb;
+    const TO* gn = (const TO*)a.dy + n * a.S * a.C;
+    const int CV = a.C / V;
+    for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+      const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+      const GnPlace p = gn_place(cw);
+      float s[V], t[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = t[j] = 0.f;
-    if (p.on) {
-      const int c = (c0 + p.col) * V;
-      GnChan<V, GV> k;
-      k.load(a, n, c);
+      for (int j = 0; j < V; ++j) s[j] = t[j] = 0.f;
+      if (p.on) {
+        const int c = (c0 + p.col) * V;
+        GnChan<V, GV> k;
+        k.load(a, n, c);
 #pragma unroll 2
-      for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
-        float v[V], g[V];
-        ld_elems<TI, V>(xn + r * a.xs + c, v);
-        ld_elems<TO, V>(gn + r * a.C + c, g);
+        for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
+          float v[V], g[V];
+          ld_elems<TI, V>(xn + r * a.xs + c, v);
+          ld_elems<TO, V>(gn + r * a.C + c, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float xh = k.xhat(j, v[j]);
-          const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
-          s[j] += dz;
-          t[j] = fmaf(dz, xh, t[j]);
+          for (int j = 0; j < V; ++j) {
+            const float xh = k.xhat(j, v[j]);
+            const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
+            s[j] += dz;
+            t[j] = fmaf(dz, xh, t[j]);
+          }
         }
       }
+      gn_fold_rows<float, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, t, p, cw);
     }
-    gn_fold_rows<float, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, t, p, cw);
-  }
-  __syncthreads();
-  float* cp = a.cpart + (long)blockIdx.x * a.C * 2;
-  for (int c = threadIdx.x; c < a.C; c += GN_NT) {
-    cp[2 * c] = sums[c];
-    cp[2 * c + 1] = sums[a.C + c];
-  }
-  for (int g = threadIdx.x; g < a.G; g += GN_NT) {
-    double s = 0.0, t = 0.0;
-    for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
-      const double w = a.w ? a.w[c] : 1.0;
-      s += w * sums[c];
-      t += w * sums[a.C + c];
+    __syncthreads();
+    float* cp = a.cpart + part * a.C * 2;
+    for (int c = threadIdx.x; c < a.C; c += GN_NT) {
+      cp[2 * c] = sums[c];
+      cp[2 * c + 1] = sums[a.C + c];
     }
-    double* o = a.gpart + ((long)blockIdx.x * a.G + g) * 2;
-    o[0] = s;
-    o[1] = t;
+    for (int g = threadIdx.x; g < a.G; g += GN_NT) {
+      double s = 0.0, t = 0.0;
+      for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
+        const double w = a.w ? a.w[c] : 1.0;
+        s += w * sums[c];
+        t += w * sums[a.C + c];
+      }
+      double* o = a.gpart + (part * a.G + g) * 2;
+      o[0] = s;
+      o[1] = t;
+    }
   }
 }
 
 constexpr int GN_FC = 4;  // channels of a finishing workgroup: 4 x 64 threads share the partial sums of 4 channels
-// workgroups 0 .. N * G / 4 (rounded up): <w dz>, <w dz xhat> of 4 (sample, group) pairs, a wave each; the rest: dw and db
+// workgroups 0 .. pair_wgs - 1: <w dz>, <w dz xhat> of the (sample, group) pairs, a wave each; the rest: dw and db
 __global__ __launch_bounds__(GN_NT) void gn_bwd_finish_kernel(GnArgs a, long pair_wgs) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if ((long)blockIdx.x < pair_wgs) {
-    const long pair = (long)blockIdx.x * 4 + wave;
-    if (pair >= a.N * a.G) return;
-    const long n = pair / a.G;
-    double s, t;
-    gn_sum_parts(a.gpart + (n * a.nblk * a.G + (pair - n * a.G)) * 2, a.nblk, a.G, s, t);
-    if (lane == 0) {
-      const double m = (double)a.S * a.q;
-      a.cc[pair * 2] = (float)(s / m);
-      a.cc[pair * 2 + 1] = (float)(t / m);
+    for (long pair = (long)blockIdx.x * 4 + wave; pair < a.N * a.G; pair += pair_wgs * 4) {
+      const long n = pair / a.G;
+      double s, t;
+      gn_sum_parts(a.gpart + (n * a.nblk * a.G + (pair - n * a.G)) * 2, a.nblk, a.G, s, t);
+      if (lane == 0) {
+        const double m = (double)a.S * a.q;
+        a.cc[pair * 2] = (float)(s / m);
+        a.cc[pair * 2 + 1] = (float)(t / m);
+      }
     }
     return;
   }
@@ -356,38 +371,40 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_finish_kernel(GnArgs a, long pai
 
 template <class TI, class TO, int V, int GV>
 __global__ __launch_bounds__(GN_NT) void gn_bwd_apply_kernel(GnArgs a) {
-  const long n = blockIdx.x / a.nblk, blk = blockIdx.x - n * a.nblk;
-  const TI* xn = (const TI*)a.x + n * a.xb;
-  const TO* gn = (const TO*)a.dy + n * a.S * a.C;
-  TI* on = (TI*)a.out + n * a.S * a.C;
-  const int CV = a.C / V;
-  for (int c0 = 0; c0 < CV; c0 += GN_NT) {
-    const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
-    const GnPlace p = gn_place(cw);
-    if (!p.on) continue;
-    const int c = (c0 + p.col) * V;
-    GnChan<V, GV> k;
-    k.load(a, n, c);
-    float m1[GV], m2[GV];
+  GN_FOR_EACH_PART(a) {
+    const long n = part / a.nblk, blk = part - n * a.nblk;
+    const TI* xn = (const TI*)a.x + n * a.xb;
+    const TO* gn = (const TO*)a.dy + n * a.S * a.C;
+    TI* on = (TI*)a.out + n * a.S * a.C;
+    const int CV = a.C / V;
+    for (int c0 = 0; c0 < CV; c0 += GN_NT) {
+      const int cw = CV - c0 < GN_NT ? CV - c0 : GN_NT;
+      const GnPlace p = gn_place(cw);
+      if (!p.on) continue;
+      const int c = (c0 + p.col) * V;
+      GnChan<V, GV> k;
+      k.load(a, n, c);
+      float m1[GV], m2[GV];
 #pragma unroll
-    for (int i = 0; i < GV; ++i) {
-      const float* cc = a.cc + (n * a.G + (c + i * (V / GV)) / a.q) * 2;
-      m1[i] = cc[0];
-      m2[i] = cc[1];
-    }
-#pragma unroll 1
-    for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
-      float v[V], g[V];
-      ld_elems<TI, V>(xn + r * a.xs + c, v);
-      ld_elems<TO, V>(gn + r * a.C + c, g);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        constexpr int Q = V / GV;
-        const float xh = k.xhat(j, v[j]);
-        const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
-        v[j] = k.rstd[j / Q] * (k.w[j] * dz - m1[j / Q] - xh * m2[j / Q]);
+      for (int i = 0; i < GV; ++i) {
+        const float* cc = a.cc + (n * a.G + (c + i * (V / GV)) / a.q) * 2;
+        m1[i] = cc[0];
+        m2[i] = cc[1];
       }
-      st_elems<TI, V>(on + r * a.C + c, v);
+#pragma unroll 1
+      for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
+        float v[V], g[V];
+        ld_elems<TI, V>(xn + r * a.xs + c, v);
+        ld_elems<TO, V>(gn + r * a.C + c, g);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          constexpr int Q = V / GV;
+          const float xh = k.xhat(j, v[j]);
+          const float dz = gn_dact(k.z(j, xh), g[j], a.act, a.slope);
+          v[j] = k.rstd[j / Q] * (k.w[j] * dz - m1[j / Q] - xh * m2[j / Q]);
+        }
+        st_elems<TI, V>(on + r * a.C + c, v);
+      }
     }
   }
 }
@@ -420,49 +437,51 @@ __device__ __forceinline__ void gn_block_sum(double& s, double& t, double* red) 
 template <class TI, class TO, int V>
 __global__ __launch_bounds__(GN_SNT) void gn_small_fwd_kernel(GnArgs a) {
   __shared__ double red[2 * GN_SNT / 64];
-  const long n = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x - n * a.G), cw = a.q / V;
-  const GnPlace p = gn_place<GN_SNT>(cw);
-  const int c = g * a.q + p.col * V;
-  const TI* x = (const TI*)a.x + n * a.xb + c;
-  double s = 0.0, sq = 0.0;
-  if (p.on) {
+  for (long pair = blockIdx.x; pair < a.N * a.G; pair += gridDim.x) {
+    const long n = pair / a.G;
+    const int g = (int)(pair - n * a.G), cw = a.q / V;
+    const GnPlace p = gn_place<GN_SNT>(cw);
+    const int c = g * a.q + p.col * V;
+    const TI* x = (const TI*)a.x + n * a.xb + c;
+    double s = 0.0, sq = 0.0;
+    if (p.on) {
+#pragma unroll 4
+      for (long r = p.rr; r < a.S; r += p.R) {
+        float v[V];
+        ld_elems<TI, V>(x + r * a.xs, v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double d = (double)v[j];
+          s += d;
+          sq = fma(d, d, sq);
+        }
+      }
+    }
+    gn_block_sum(s, sq, red);
+    const double m = (double)a.S * a.q, mean = s / m;
+    double var = sq / m - mean * mean;
+    if (var < 0.0) var = 0.0;  // NaN stays
+    const float mu = (float)mean, rstd = (float)(1.0 / sqrt(var + (double)a.eps));
+    if (threadIdx.x == 0) {
+      a.stats[pair * 2] = mu;
+      a.stats[pair * 2 + 1] = rstd;
+    }
+    if (!p.on) continue;
+    float w[V], b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      w[j] = a.w ? a.w[c + j] : 1.f;
+      b[j] = a.b ? a.b[c + j] : 0.f;
+    }
+    TO* y = (TO*)a.out + n * a.S * a.C + c;
 #pragma unroll 4
     for (long r = p.rr; r < a.S; r += p.R) {
       float v[V];
       ld_elems<TI, V>(x + r * a.xs, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double d = (double)v[j];
-        s += d;
-        sq = fma(d, d, sq);
-      }
+      for (int j = 0; j < V; ++j) v[j] = gn_act(fmaf((v[j] - mu) * rstd, w[j], b[j]), a.act, a.slope);
+      st_elems<TO, V>(y + r * a.C, v);
     }
-  }
-  gn_block_sum(s, sq, red);
-  const double m = (double)a.S * a.q, mean = s / m;
-  double var = sq / m - mean * mean;
-  if (var < 0.0) var = 0.0;  // NaN stays
-  const float mu = (float)mean, rstd = (float)(1.0 / sqrt(var + (double)a.eps));
-  if (threadIdx.x == 0) {
-    a.stats[(long)blockIdx.x * 2] = mu;
-    a.stats[(long)blockIdx.x * 2 + 1] = rstd;
-  }
-  if (!p.on) return;
-  float w[V], b[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    w[j] = a.w ? a.w[c + j] : 1.f;
-    b[j] = a.b ? a.b[c + j] : 0.f;
-  }
-  TO* y = (TO*)a.out + n * a.S * a.C + c;
-#pragma unroll 4
-  for (long r = p.rr; r < a.S; r += p.R) {
-    float v[V];
-    ld_elems<TI, V>(x + r * a.xs, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = gn_act(fmaf((v[j] - mu) * rstd, w[j], b[j]), a.act, a.slope);
-    st_elems<TO, V>(y + r * a.C, v);
   }
 }
 
@@ -531,8 +550,8 @@ constexpr long GN_TARGET = 1024;  // workgroups of a launch that sums
 constexpr long GN_TARGET_APPLY = 4096;  // of one that writes (1 024: 119 us instead of 89 for the forward at 2 x 128^3 x 32 f16)
 // Workgroups of a sample: enough to fill the chip, with at least 8 passes over the rows that their threads cover at once.  The rows
 // are dealt out in turn, so that the chip reads one moving window: runs of rows a workgroup lie a power of two apart on the usual
-// sizes, and their streams then meet in the same memory channels (stats / apply / reduce at 2 x 128^3 x 32 f16: 63 / 92 / 140 us that way, 58 /
-// 89 / 130 in turn).
+// sizes, and their streams then meet in the same memory channels (stats / apply / reduce at 2 x 128^3 x 32 f16: 63 / 92 / 140 us
+// that way, 58 / 89 / 130 in turn).
 inline void gn_split(GnArgs& a, int V, long target) {
   const int CV = a.C / V;
   const long R = CV >= GN_NT ? 1 : GN_NT / CV;
@@ -547,6 +566,7 @@ inline bool gn_small(long N, long S, int q, bool bwd) {
   if (q > GN_SNT) return false;
   return bwd ? N <= GN_SMALL_N && N * S * q <= GN_SMALL_BWD : S * q <= GN_SMALL_FWD;
 }
+inline dim3 gn_grid(long wgs) { return dim3((unsigned)(wgs < GN_MAX_WG ? wgs : GN_MAX_WG)); }
 inline long gn_align(long v) { return (v + 255) & ~255L; }
 // layout of the workspace, the same whatever V a call's alignment allows
 struct GnWs {
@@ -571,12 +591,12 @@ static int gn_large_fwd(GnArgs a, hipStream_t s) {
   const int lds = (GN_NT * V + a.C) * 2 * 8;
   hipError_t e = ensure_dyn_lds((const void*)gn_stats_kernel<TI, V>, lds, cache);
   if (e != hipSuccess) return (int)e;
-  NNZ_LAUNCH((gn_stats_kernel<TI, V>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH((gn_stats_kernel<TI, V>), gn_grid(a.N * a.nblk), dim3(GN_NT), lds, s, a);
   NNZ_LAUNCH_CHECK();
-  NNZ_LAUNCH(gn_stats_finish_kernel, dim3((unsigned)(a.N * a.G)), dim3(64), 0, s, a);
+  NNZ_LAUNCH(gn_stats_finish_kernel, gn_grid(a.N * a.G), dim3(64), 0, s, a);
   NNZ_LAUNCH_CHECK();
   gn_split(a, V, GN_TARGET_APPLY);
-  NNZ_LAUNCH((gn_apply_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), 0, s, a);
+  NNZ_LAUNCH((gn_apply_kernel<TI, TO, V, GV>), gn_grid(a.N * a.nblk), dim3(GN_NT), 0, s, a);
   NNZ_LAUNCH_CHECK();
   return NNZ_OK;
 }
@@ -587,20 +607,20 @@ static int gn_large_bwd(GnArgs a, hipStream_t s) {
   const int lds = (GN_NT * V + a.C) * 2 * 4;
   hipError_t e = ensure_dyn_lds((const void*)gn_bwd_reduce_kernel<TI, TO, V, GV>, lds, cache);
   if (e != hipSuccess) return (int)e;
-  NNZ_LAUNCH((gn_bwd_reduce_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), lds, s, a);
+  NNZ_LAUNCH((gn_bwd_reduce_kernel<TI, TO, V, GV>), gn_grid(a.N * a.nblk), dim3(GN_NT), lds, s, a);
   NNZ_LAUNCH_CHECK();
-  const long pair_wgs = (a.N * a.G + 3) / 4;
+  const long pairs4 = (a.N * a.G + 3) / 4, pair_wgs = pairs4 < GN_MAX_WG ? pairs4 : GN_MAX_WG;
   NNZ_LAUNCH(gn_bwd_finish_kernel, dim3((unsigned)(pair_wgs + (a.C + GN_FC - 1) / GN_FC)), dim3(GN_NT), 0, s, a, pair_wgs);
   NNZ_LAUNCH_CHECK();
   gn_split(a, V, GN_TARGET_APPLY);
-  NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V, GV>), dim3((unsigned)(a.N * a.nblk)), dim3(GN_NT), 0, s, a);
+  NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V, GV>), gn_grid(a.N * a.nblk), dim3(GN_NT), 0, s, a);
   NNZ_LAUNCH_CHECK();
   return NNZ_OK;
 }
 template <class TI, class TO, int V>
 static int gn_run(const GnArgs& a, bool bwd, hipStream_t s) {
   if (gn_small(a.N, a.S, a.q, bwd)) {
-    const dim3 grid((unsigned)(bwd ? a.G : a.N * a.G));
+    const dim3 grid = gn_grid(bwd ? a.G : a.N * a.G);
     if (bwd && a.q % V == 0) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, V>), grid, dim3(GN_SNT), 0, s, a);
     else if (bwd) NNZ_LAUNCH((gn_small_bwd_kernel<TI, TO, 1>), grid, dim3(GN_SNT), 0, s, a);
     else if (a.q % V == 0) NNZ_LAUNCH((gn_small_fwd_kernel<TI, TO, V>), grid, dim3(GN_SNT), 0, s, a);
@@ -637,7 +657,7 @@ static int gn_go(const GnArgs& a, int ti, int to, bool bwd, hipStream_t s) {
   return NNZ_EINVAL;
 }
 static bool gn_shape_ok(long N, long S, int C, int G) {
-  return N >= 1 && S >= 1 && C >= 1 && C <= GN_MAX_C && G >= 1 && C % G == 0 && N <= (1L << 28) / G && S <= (1L << 40) / C / N;
+  return N >= 1 && S >= 1 && C >= 1 && C <= GN_MAX_C && G >= 1 && C % G == 0 && N <= (1L << 40) / C && S <= (1L << 40) / C / N;
 }
 
 }  // namespace nnz

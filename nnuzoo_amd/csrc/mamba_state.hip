@@ -48,7 +48,8 @@ struct RowVec<T, 1> {
 };
 
 // A thread: V adjacent channels, tt consecutive tokens, the window in registers.  Bound by HBM (x in, y out); a load in front of every
-// token's stores waited for those as well (53 us), loads U tokens ahead: 46 us = 4.4 TB/s at 2 x 262144 x 96 f16, W = 4.
+// token's stores waited for those as well; with loads U tokens ahead 51 us = 3.9 TB/s at 2 x 262144 x 96 f16, W = 4, where x is one
+// half of rows of 384 bytes, so that a third of every second line fetched is not x.
 template <class T, int W, int V>
 __global__ __launch_bounds__(256) void conv_prompt_kernel(ConvStateArgs a) {
   const int CV = a.D / V;
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(256) void conv_prompt_kernel(ConvStateArgs a) {
   for (int t = te > t0 ? te : t0; t < t1; ++t) st_elems<T, V>(y + (long)t * a.D, zero);
 }
 
-// one token: a thread per (sequence, channel)
+// One token: a thread per (sequence, channel); 3 us, the smallest launch's time, at the sizes of a decoder's step.
 template <class T, int W>
 __global__ __launch_bounds__(256) void conv_token_kernel(ConvStateArgs a) {
   const long id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -175,7 +176,7 @@ static int conv_state_run(ConvStateArgs a, bool token, hipStream_t s) {
     NNZ_LAUNCH_CHECK();
     return NNZ_OK;
   }
-  constexpr int FULL = 4;   // 8 f16 a thread: 178 registers at W = 4 instead of 100, 50 us instead of 46 at 2 x 262144 x 96
+  constexpr int FULL = 4;   // 8 f16 a thread: 178 registers at W = 4 instead of 100, 57 us instead of 51 at 2 x 262144 x 96
   const bool vec = a.D % FULL == 0 && a.xb % FULL == 0 && a.xt % FULL == 0 &&
                    (((uintptr_t)a.x | (uintptr_t)a.y) & (FULL * sizeof(T) - 1)) == 0;
   const int CV = vec ? a.D / FULL : a.D;
@@ -183,7 +184,7 @@ static int conv_state_run(ConvStateArgs a, bool token, hipStream_t s) {
   // a sequence's first chunk may need the state, for its thread writes the new one (8 >= W - 1)
   a.tt = (long)CV * a.B * ((a.L + 15) / 16) < 256L * 512 ? 8 : 16;
   const long wg = ((long)CV * a.B * ((a.L + a.tt - 1) / a.tt) + 255) / 256;
-  if (wg > 0x7FFFFFFFL) return NNZ_EINVAL;
+  if (wg >= 1L << 24) return NNZ_EINVAL;   // 2^32 threads
   if (vec) NNZ_LAUNCH((conv_prompt_kernel<T, W, FULL>), dim3((unsigned)wg), dim3(256), 0, s, a);
   else NNZ_LAUNCH((conv_prompt_kernel<T, W, 1>), dim3((unsigned)wg), dim3(256), 0, s, a);
   NNZ_LAUNCH_CHECK();
@@ -273,7 +274,8 @@ __device__ __forceinline__ ElemVec<T, 2> ld_pair(const T* p, bool aligned, int s
 
 // 4 lanes share CPL channels and hold N / 4 states of each; a workgroup has nch = 16 CPL channels a wave of one group and walks
 // its tokens in tiles: every (token, channel) of a tile is loaded and turned into D_t, D_t x_t once, B and C are widened once, all
-// through LDS.  Bound by the vector unit: per token, channel and state a 2^x (quarter rate), two products and two FMAs.
+// through LDS.  Bound by the vector unit: per token, channel and state a 2^x (quarter rate), two products and two FMAs - 32 cycles a
+// wave of 64 states, 165 us for one pass at 2 x 262144 x 96, N = 16; measured there (f16): summaries 189 us, joining 21, outputs 261.
 // MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks that run in parallel: MODE 1 leaves
 // every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)),
 // scan_join_kernel turns the summaries into entry states, MODE 2 runs the chunks from those.
@@ -509,33 +511,36 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
   }
 }
 
-// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A lane per (channel, state); where there
-// are many chunks 16 waves share them: each joins its own run, then starts again from the runs before it.
-template <int N, int SJ_SEG>
-__global__ __launch_bounds__(64 * SJ_SEG) void scan_join_kernel(ScanStateArgs a) {
-  __shared__ float s_p[SJ_SEG][64], s_h[SJ_SEG][64];
-  const int lane = threadIdx.x & 63, seg = threadIdx.x >> 6, b = blockIdx.y;
-  const long dn = (long)a.D * N, i = (long)blockIdx.x * 64 + lane;
+// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A thread per (channel, state); where there
+// are many chunks SEG threads share them: each joins its own run, then starts again from the runs before it (1 261 chunks of
+// 2 x 96 x 16 states: 21 us with 64 runs, 26 us with 16).
+template <int N, int LN, int SEG>
+__global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
+  __shared__ float s_p[SEG][LN], s_h[SEG][LN];
+  const int lane = threadIdx.x % LN, seg = threadIdx.x / LN, b = blockIdx.y;
+  const long dn = (long)a.D * N, i = (long)blockIdx.x * LN + lane;
   const long at = i < dn ? i : dn - 1;
   const int d = (int)(at / N), hd = d / a.rep;
   const float A2 = decay2(a.a_n ? a.A[(long)hd * N + at % N] : a.A[hd]);
-  const int per = (a.chunks + SJ_SEG - 1) / SJ_SEG;
+  const int per = (a.chunks + SEG - 1) / SEG;
   const int c0 = seg * per, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
   float* ph = a.part_h + (long)b * dn + at;
   const float* pd = a.part_d + (long)b * a.D + d;
   const long hs = (long)a.B * dn, ds = (long)a.B * a.D;
-  float p = 0.f, h = 0.f;
-#pragma unroll 8
-  for (int c = c0; c < c1; ++c) {
-    const float sum = pd[c * ds];
-    h = fmaf(__builtin_amdgcn_exp2f(sum * A2), h, ph[c * hs]);
-    p += sum;
-  }
-  s_p[seg][lane] = p;
-  s_h[seg][lane] = h;
-  __syncthreads();
   float e = a.state ? a.state[(long)b * a.sb + at] : 0.f;
-  for (int s = 0; s < seg; ++s) e = fmaf(__builtin_amdgcn_exp2f(s_p[s][lane] * A2), e, s_h[s][lane]);
+  if constexpr (SEG > 1) {
+    float p = 0.f, h = 0.f;
+#pragma unroll 8
+    for (int c = c0; c < c1; ++c) {
+      const float sum = pd[c * ds];
+      h = fmaf(__builtin_amdgcn_exp2f(sum * A2), h, ph[c * hs]);
+      p += sum;
+    }
+    s_p[seg][lane] = p;
+    s_h[seg][lane] = h;
+    __syncthreads();
+    for (int s = 0; s < seg; ++s) e = fmaf(__builtin_amdgcn_exp2f(s_p[s][lane] * A2), e, s_h[s][lane]);
+  }
   if (i >= dn) return;
 #pragma unroll 8
   for (int c = c0; c < c1; ++c) {
@@ -545,7 +550,8 @@ __global__ __launch_bounds__(64 * SJ_SEG) void scan_join_kernel(ScanStateArgs a)
   }
 }
 
-// one token: 4 lanes a channel
+// One token: 4 lanes a channel, each its N / 4 states in one access.  Bound by HBM (the states in and out): 128 x 1536 x 16: 11.8 us =
+// 2.3 TB/s, of which 3.5 us is what the smallest launch takes.
 template <class T, int N>
 __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
   constexpr int NS = N / 4;
@@ -629,9 +635,9 @@ static int scan_prompt_run(const ScanStateArgs& a, hipStream_t s) {
     if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 2>, lds, c2)) != hipSuccess) return (int)e;
     NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), grid, block, lds1, s, a);
     NNZ_LAUNCH_CHECK();
-    const dim3 jg((unsigned)(((long)a.D * N + 63) / 64), a.B);
-    if (a.chunks > 64) NNZ_LAUNCH((scan_join_kernel<N, 16>), jg, dim3(64 * 16), 0, s, a);
-    else NNZ_LAUNCH((scan_join_kernel<N, 1>), jg, dim3(64), 0, s, a);
+    const long dn = (long)a.D * N;
+    if (a.chunks > 64) NNZ_LAUNCH((scan_join_kernel<N, 16, 64>), dim3((unsigned)((dn + 15) / 16), a.B), dim3(1024), 0, s, a);
+    else NNZ_LAUNCH((scan_join_kernel<N, 64, 1>), dim3((unsigned)((dn + 63) / 64), a.B), dim3(64), 0, s, a);
     NNZ_LAUNCH_CHECK();
     NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 2>), grid, block, lds, s, a);
   }
@@ -642,7 +648,7 @@ template <class T, int N>
 static int scan_state_run(const ScanStateArgs& a, int cpl, bool token, hipStream_t s) {
   if (token) {
     const long wg = ((long)a.B * a.D * 4 + 255) / 256;
-    if (wg > 0x7FFFFFFFL) return NNZ_EINVAL;
+    if (wg >= 1L << 24) return NNZ_EINVAL;   // 2^32 threads
     NNZ_LAUNCH((scan_token_kernel<T, N>), dim3((unsigned)wg), dim3(256), 0, s, a);
     NNZ_LAUNCH_CHECK();
     return NNZ_OK;
@@ -691,7 +697,7 @@ extern "C" int nnz_causal_conv1d_token(const void* x, int type, long x_batch_str
                                        long state_column_stride, const void* active, int B, int D, int W, int silu,
                                        void* stream) {
   using namespace nnz;
-  if (!x || !weight || !y || !conv_state || B < 1 || D < 1 || (long)B * D > (1L << 38) || !elem_ok(state_type)) return NNZ_EINVAL;
+  if (!x || !weight || !y || !conv_state || B < 1 || D < 1 || (long)B * D > 0xFFFFFF00L || !elem_ok(state_type)) return NNZ_EINVAL;
   ConvStateArgs a = {};
   a.x = x; a.w = weight; a.bias = bias; a.y = y; a.st = conv_state; a.len = active;
   a.xb = x_batch_stride; a.sb = state_batch_stride; a.sd = state_channel_stride; a.sw = state_column_stride;

@@ -59,6 +59,13 @@ def test_many_workgroups(hip_lib, dt, N, S, C, groups):
 
 
 @gpu
+def test_more_groups_than_a_grid_has_workgroups(hip_lib):
+    """600 000 samples x 8 groups: past 2^22 workgroups each takes several groups"""
+    x, w, b, dy = _data(600000, 2, 8, torch.float16, seed=14)
+    _check(x, 8, w, b, dy, "silu", eps=1e-2)
+
+
+@gpu
 @pytest.mark.parametrize("affine", [(False, False), (True, False), (False, True)])
 def test_without_affine_parameters(hip_lib, affine):
     x, w, b, dy = _data(2, 50, 16, torch.float32, seed=3)

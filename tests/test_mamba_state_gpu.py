@@ -204,6 +204,18 @@ def test_scan_of_several_chunks_ragged(hip_lib, dt, d, L, join):
 
 
 @gpu
+def test_scan_of_many_chunks(hip_lib):
+    """more than 64 chunks: runs of them are joined side by side"""
+    v = _scan_data(2, 5000, 8, 8, 1, 4, "f32", seed=11)
+    v["dt_bias"] -= 3      # slow decays, so that far chunks still matter
+    lengths = [5000, 4163]
+    y, st = _scan_got(v, lengths=torch.tensor(lengths, dtype=torch.int32).cuda())
+    want, new = _scan_want(v, lengths, join=64)
+    close(y, *want, "y")
+    close(st, *new, "state")
+
+
+@gpu
 def test_scan_repeats_bit_for_bit(hip_lib):
     v = _scan_data(2, 3000, 24, 24, 1, 16, "f16", seed=9)
     first = _scan_got(v)
