@@ -207,6 +207,23 @@ def test_module_and_evaluation(hip_lib):
 
 
 @gpu
+def test_gradient_of_the_residual_alone_and_of_one_tensor_twice(hip_lib):
+    from nnuzoo_amd.dropout import dropout_add, dropout_state
+    state = dropout_state(2, "cuda")
+    x, r = torch.randn(70, device="cuda"), torch.randn(70, device="cuda", requires_grad=True)
+    dr, = torch.autograd.grad(dropout_add(x, r, 0.5, state).sum(), r)
+    assert torch.equal(dr, torch.ones_like(r))
+    both, = torch.autograd.grad(dropout_add(r, r, 0.5, state).sum(), r)
+    kept = dropout_kept(2, 0, 0, 70, 0.5).cuda()
+    assert torch.equal(both, torch.where(kept, 3.0, 1.0))
+    view = torch.randn(4, 6, device="cuda").t()                       # gradients of strided inputs and outputs
+    v = view.clone().requires_grad_(True)
+    y = dropout_add(v.t(), v.t(), 0.5, state)
+    y.t().backward(torch.ones(6, 4, device="cuda"))
+    assert torch.equal(v.grad, torch.where(dropout_kept(2, 0, 0, 24, 0.5).view(4, 6).cuda(), 3.0, 1.0).t())
+
+
+@gpu
 def test_empty(hip_lib):
     from nnuzoo_amd.dropout import dropout, dropout_add, dropout_state
     x = torch.zeros(0, 4, device="cuda", requires_grad=True)

@@ -163,6 +163,26 @@ def test_constant_rows_and_empty_tensors(hip_lib):
 
 
 @gpu
+def test_rows_without_spatial_axes_and_single_gradients(hip_lib):
+    """x (N, C); gradients of x alone, of the parameters alone, of an expanded dy"""
+    from nnuzoo_amd.group_norm import group_norm_act
+    x, w, b, _ = _data(37, 1, 24, torch.float32, seed=13)
+    dy = torch.full_like(x, 0.5)
+    want = oracle(x, 3, w, b, 1e-5, "silu", SLOPE, dy)
+    ins = [t.cuda() for t in (x[:, 0], w, b)]
+    for need in ((0,), (1,), (2,), (1, 2), (0, 1, 2)):
+        args = [t.clone().requires_grad_(i in need) for i, t in enumerate(ins)]
+        y = group_norm_act(args[0], 3, args[1], args[2], 1e-5, "silu")
+        close(y[:, None], *want["y"], "y")
+        (y * 0.5).sum().backward()
+        for i, name in enumerate(("dx", "dw", "db")):
+            if i in need:
+                close(args[i].grad.reshape(want[name][0].shape), *want[name], name)
+            else:
+                assert args[i].grad is None
+
+
+@gpu
 def test_bit_identical_runs_and_side_stream(hip_lib):
     from nnuzoo_amd.group_norm import group_norm_act
     x, w, b, dy = (t.cuda() for t in _data(2, 5000, 32, torch.float16, seed=10))
