@@ -2,14 +2,14 @@
 //   z = (x - mu[n,g]) * r[n,g] * w[c] + b[c],  y = act(z),  mu / r over the S positions and C / G channels of a group;
 //   dz = dy act'(z),  db = sum dz,  dw = sum dz xhat,  dx = r (w dz - <w dz> - xhat <w dz xhat>)  with <.> the group's mean.
 // Bound by HBM: a group does not fit on chip, so forward reads x twice and writes y, backward reads x and dy twice and writes dx.
-// 2 x 128^3 x 32 f16 (268 MB a tensor), SiLU: sums 59 us (4.5 TB/s), write pass 89 (6.0), backward sums 126 (4.3, the logistic
-// function's share shows), write pass 150 (5.4), finishing launches 5 each.
+// 2 x 128^3 x 32 f16 (268 MB a tensor), SiLU: sums 65 us (4.1 TB/s), write pass 90 (6.0), backward sums 131 (4.1, the logistic
+// function's share shows), write pass 151 (5.3), finishing launches 5 each.
 //
 // A thread owns V consecutive channels (16 bytes) and walks the rows, a workgroup owns a run of rows of one sample: every access
-// is a run of whole rows whatever the group width, and the group's members meet only after the rows are summed.  Sums of the
-// forward are kept in fp64 (the vector rate of fp64 FMA is that of plain fp32 here, and E[x^2] - mu^2 then loses nothing
-// that fp32 statistics could hold, whatever mu / sigma is); partial sums go to a workspace and are added in a fixed order, so
-// results are bit-identical from run to run.  No atomics.
+// is a run of whole rows whatever the group width, and the group's members meet only after the rows are summed.  The forward's sums
+// are fp64 (whose vector rate is that of plain fp32 here), so that E[x^2] - mu^2 loses nothing that fp32 statistics could hold,
+// whatever mu / sigma is.  Partial sums go through a workspace and are added in a fixed order: results are bit-identical from run
+// to run.  No atomics.
 #include "elem_io.hpp"
 
 namespace nnz {
@@ -127,10 +127,32 @@ __device__ __forceinline__ void gn_fold_rows(A* stage, A* dst_s, A* dst_t, const
   }
 }
 
-// A thread's sums are taken about its own first value of each channel, in fp32, and become sums about 0 in fp64 once its rows are
-// done: sum (x - k)^2 is at most a small multiple of what these rows and k add to the variance, so the rounding of fp32 sums of
-// m terms costs m * 2^-24 of the variance at the very most, whatever mu / sigma is.  (At 2 x 128^3 x 32 f16: 58 us, 4.6 TB/s;
-// plain reads reach 6.4 here.)
+// per-group sums of two per-channel sums [2][C], weighted by w, in fp64 and in a fixed order: up to 64 lanes a group
+template <class A>
+__device__ __forceinline__ void gn_fold_groups(const GnArgs& a, const A* sums, const float* w, double* out) {
+  int lp = 1;
+  while (2 * lp <= a.q && lp < 64) lp *= 2;
+  const int li = threadIdx.x & (lp - 1);
+  for (int g = threadIdx.x / lp; g < a.G; g += GN_NT / lp) {
+    double u = 0.0, v = 0.0;
+    for (int c = g * a.q + li; c < (g + 1) * a.q; c += lp) {
+      const double k = w ? w[c] : 1.0;
+      u = fma(k, (double)sums[c], u);
+      v = fma(k, (double)sums[a.C + c], v);
+    }
+    for (int o = lp / 2; o > 0; o >>= 1) {
+      u += __shfl_xor(u, o, 64);
+      v += __shfl_xor(v, o, 64);
+    }
+    if (li == 0) {
+      out[2 * g] = u;
+      out[2 * g + 1] = v;
+    }
+  }
+}
+
+// fp64 throughout: fp32 sums about a thread's own first value took as long (the kernel waits for memory) and are at the mercy of
+// that value.
 template <class TI, int V>
 __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
   extern __shared__ __attribute__((aligned(16))) double gn_lds_d[];
@@ -146,46 +168,24 @@ __global__ __launch_bounds__(GN_NT) void gn_stats_kernel(GnArgs a) {
       double s[V], sq[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) s[j] = sq[j] = 0.0;
-      const long first = blk * p.R + p.rr, hop = (long)a.nblk * p.R;
-      if (p.on && first < a.S) {
-        const TI* xc = xn + (long)(c0 + p.col) * V + first * a.xs;
-        const long step = hop * a.xs;
-        float k[V], d1[V], d2[V];
-        ld_elems<TI, V>(xc, k);
-#pragma unroll
-        for (int j = 0; j < V; ++j) d1[j] = d2[j] = 0.f;
-        const long cnt = (a.S - first + hop - 1) / hop;
+      if (p.on) {
+        const TI* xc = xn + (long)(c0 + p.col) * V;
 #pragma unroll 2
-        for (long i = 1; i < cnt; ++i) {
+        for (long r = blk * p.R + p.rr; r < a.S; r += (long)a.nblk * p.R) {
           float v[V];
-          ld_elems<TI, V>(xc + i * step, v);
+          ld_elems<TI, V>(xc + r * a.xs, v);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float d = v[j] - k[j];
-            d1[j] += d;
-            d2[j] = fmaf(d, d, d2[j]);
+            const double d = (double)v[j];
+            s[j] += d;
+            sq[j] = fma(d, d, sq[j]);
           }
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const double kd = k[j], s1 = d1[j], m = (double)cnt;
-          s[j] = fma(m, kd, s1);
-          sq[j] = fma(kd, fma(m, kd, 2.0 * s1), (double)d2[j]);
         }
       }
       gn_fold_rows<double, V>(stage, sums + c0 * V, sums + a.C + c0 * V, s, sq, p, cw);
     }
     __syncthreads();
-    for (int g = threadIdx.x; g < a.G; g += GN_NT) {
-      double s = 0.0, sq = 0.0;
-      for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
-        s += sums[c];
-        sq += sums[a.C + c];
-      }
-      double* o = a.gpart + (part * a.G + g) * 2;
-      o[0] = s;
-      o[1] = sq;
-    }
+    gn_fold_groups(a, sums, nullptr, a.gpart + part * a.G * 2);
   }
 }
 
@@ -309,17 +309,7 @@ __global__ __launch_bounds__(GN_NT) void gn_bwd_reduce_kernel(GnArgs a) {
       cp[2 * c] = sums[c];
       cp[2 * c + 1] = sums[a.C + c];
     }
-    for (int g = threadIdx.x; g < a.G; g += GN_NT) {
-      double s = 0.0, t = 0.0;
-      for (int c = g * a.q; c < (g + 1) * a.q; ++c) {
-        const double w = a.w ? a.w[c] : 1.0;
-        s += w * sums[c];
-        t += w * sums[a.C + c];
-      }
-      double* o = a.gpart + (part * a.G + g) * 2;
-      o[0] = s;
-      o[1] = t;
-    }
+    gn_fold_groups(a, sums, a.w, a.gpart + part * a.G * 2);
   }
 }
 

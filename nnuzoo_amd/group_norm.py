@@ -8,7 +8,8 @@ gradient.
   norm_act(norm, act, x)                                                            act(norm(x)) of two modules on either path
 
 fp32 / fp16 / bf16 in; the output has the input's type, or fp32 under autocast (group_norm is on autocast's fp32 list).
-Statistics are fp64 sums, everything else is computed in fp32 and rounded once.  Results are bit-identical from run to run."""
+Statistics are fp64 sums, everything else is computed in fp32 and rounded once.  Results are bit-identical from run to run.
+There is no second derivative and no CPU path."""
 from __future__ import annotations
 
 from typing import Optional
@@ -27,14 +28,16 @@ def _rows(x: torch.Tensor):
     """(x or its contiguous copy, batch stride, row stride): rows of C adjacent elements, evenly spaced within a sample"""
     C = x.shape[-1]
     if x.stride(-1) == 1 or C == 1:
-        step = x.stride(-2) if x.dim() > 2 else C
-        want = step
+        step = want = None
         for d in range(x.dim() - 2, 0, -1):
-            if x.shape[d] != 1 and x.stride(d) != want:
-                break
-            want *= x.shape[d]
+            if x.shape[d] != 1:
+                if step is None:
+                    step = want = x.stride(d)
+                elif x.stride(d) != want:
+                    break
+                want *= x.shape[d]
         else:
-            return x, x.stride(0), step
+            return x, x.stride(0), C if step is None else step
     x = x.contiguous()
     return x, x.numel() // max(1, x.shape[0]), C
 
@@ -44,19 +47,19 @@ class _GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, eps, act, slope, out_dtype):
         dev = x.device
         x, xb, xs = _rows(x)
-        N, C = x.shape[0], x.shape[-1]
         y = torch.empty(x.shape, dtype=out_dtype, device=dev)
-        ctx.cfg = (xb, xs, groups, act, slope)
-        if y.numel() == 0:
-            ctx.save_for_backward(x, weight, bias, None)
-            return y
-        S = x.numel() // (N * C)
-        ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 0)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-        stats = torch.empty(2 * N * groups, dtype=torch.float32, device=dev)
-        launch("nnz_group_norm_act_forward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, ptr(weight), ptr(bias), y.data_ptr(),
-               ELEM[out_dtype], stats.data_ptr(), ptr(ws), ws_bytes, N, S, C, groups, eps, act, slope)
-        ctx.save_for_backward(x, weight, bias, stats)
+        N, C = x.shape[0], x.shape[-1]
+        stats = None
+        if y.numel():
+            S = x.numel() // (N * C)
+            ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 0)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+            stats = torch.empty(2 * N * groups, dtype=torch.float32, device=dev)
+            launch("nnz_group_norm_act_forward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, ptr(weight), ptr(bias), y.data_ptr(),
+                   ELEM[out_dtype], stats.data_ptr(), ptr(ws), ws_bytes, N, S, C, groups, eps, act, slope)
+            ctx.cfg = (xb, xs, N, S, C, groups, act, slope)
+        ctx.save_for_backward(x, weight, bias)
+        ctx.stats = stats       # of this node's own making: neither input nor output
         return y
 
     @staticmethod
@@ -65,26 +68,24 @@ class _GroupNormActFn(torch.autograd.Function):
             return _backward(ctx, dy)
         with torch.no_grad():
             grads = _backward(ctx, dy)
-        return first_order("group_norm_act", grads, (dy, *ctx.saved_tensors[:3]))
+        return first_order("group_norm_act", grads, (dy, *ctx.saved_tensors))
 
 
 def _backward(ctx, dy):
-    x, weight, bias, stats = ctx.saved_tensors
-    xb, xs, groups, act, slope = ctx.cfg
-    dev, N, C = x.device, x.shape[0], x.shape[-1]
-    need_w, need_b = ctx.needs_input_grad[1], ctx.needs_input_grad[2]
-    make = torch.empty if stats is not None else torch.zeros
+    x, weight, bias = ctx.saved_tensors
+    _, need_w, need_b, *_ = ctx.needs_input_grad
+    dev, C, stats = x.device, x.shape[-1], ctx.stats
+    make = torch.zeros if stats is None else torch.empty
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     dw = make(C, dtype=torch.float32, device=dev) if need_w else None
     db = make(C, dtype=torch.float32, device=dev) if need_b else None
     if stats is not None:
+        xb, xs, N, S, C, groups, act, slope = ctx.cfg
         dy = dy.contiguous()
-        S = x.numel() // (N * C)
         ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
-               ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C,
-               groups, act, slope)
+               ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C, groups, act, slope)
     return dx, dw, db, None, None, None, None, None
 
 

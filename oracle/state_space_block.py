@@ -42,10 +42,9 @@ def _act(z, act, slope):
     return z, torch.ones_like(z), torch.ones_like(z)
 
 
-def group_norm_act(x, groups, w, b, eps, act, slope, dy, additions=512, rows=16):
+def group_norm_act(x, groups, w, b, eps, act, slope, dy, additions=512):
     """x, dy (N, S, C), w, b (C,) or None.  -> {name: (value, bound)} for y, dx, dw, db.
-    `additions`: the longest chain of fp32 additions in a sum of the backward (rows of a thread + threads of a workgroup); `rows`: that
-    of a sum of squares of the forward (taken about one of its terms, so its rounding is relative to the variance)."""
+    `additions`: the longest chain of fp32 additions in a sum of the backward (rows of a thread + threads of a workgroup)."""
     x, dy = x.double().cpu(), dy.double().cpu()
     N, S, C = x.shape
     q = C // groups
@@ -60,7 +59,7 @@ def group_norm_act(x, groups, w, b, eps, act, slope, dy, additions=512, rows=16)
     xh = (x - mean_f) * r_f
     z = xh * w + b
     # mean and r are rounded once each, then a subtraction, two products and a sum; E[x^2] - mean^2 in fp64 leaves 2^-50 of E[x^2]
-    e_var = 2.0 ** -50 * (mean_f.square() + full(var)) * r_f.square() + rows * U / 2
+    e_var = 2.0 ** -50 * (mean_f.square() + full(var)) * r_f.square()
     e_xh = U * mean_f.abs() * r_f + xh.abs() * (4 * U + e_var)
     e_z = e_xh * w.abs() + 3 * U * ((xh * w).abs() + b.abs())
     y, d, dmax = _act(z, act, slope)
