@@ -59,6 +59,16 @@ def test_many_workgroups(hip_lib, dt, N, S, C, groups):
 
 
 @gpu
+@pytest.mark.parametrize("N,S,C,groups", [(9, 16, 64, 8), (300, 4, 24, 3), (40, 30, 66, 1), (33, 64, 512, 2), (20, 400, 40, 1),
+                                          (1000, 1, 8, 8), (9000, 2, 16, 2), (3000, 5, 60, 6), (12, 100, 600, 1)])
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_many_small_samples(hip_lib, dt, N, S, C, groups):
+    """waves and workgroups that walk several samples of a group, partial weight gradients added up after them"""
+    x, w, b, dy = _data(N, S, C, DT[dt], seed=N)
+    _check(x, groups, w, b, dy, "silu", eps=1e-2)
+
+
+@gpu
 def test_more_groups_than_a_grid_has_workgroups(hip_lib):
     """600 000 samples x 8 groups: past 2^22 workgroups each takes several groups"""
     x, w, b, dy = _data(600000, 2, 8, torch.float16, seed=14)
