@@ -776,7 +776,7 @@ int nnz_dropout_backward(const void* dy, int dy_type, void* dx, int dx_type, lon
 /* ---- the state-carrying operators of the 1-D Mamba blocks, token-major (Mamba.step and inference_params,
  * nets/seg_mamba/mamba_simple.py:190-215, 357-411).  type: element type of the activations.  conv_state [B][D][W] (any strides,
  * element type state_type; NULL in the prompt form: zeros, nothing kept) and state [B][D][N] fp32 (contiguous within a sequence)
- * are updated in place.  lengths: [B] int32 / int64 device or NULL; active: [B] bytes or NULL.  W <= 8; N 4, 8, 16, 32.
+ * are updated in place.  A_form: 1 for A [H][N], 0 for A [H], + 2 where the entries are log(-A).  lengths: [B] int32 / int64 or NULL; active: [B] bytes or NULL.  W <= 8; N 4, 8, 16, 32.
  * strides (host table, elements): prompt {x batch, x token, dt batch, dt token, B batch, B token, B group, C batch, C token,
  * C group, z batch, z token}; token {x batch, dt batch, B batch, B group, C batch, C group, z batch}. */
 int nnz_causal_conv1d_prompt(const void* x, int type, long x_batch_stride, long x_token_stride, const float* weight,
@@ -788,12 +788,12 @@ int nnz_causal_conv1d_token(const void* x, int type, long x_batch_stride, const 
                             long state_column_stride, const void* active, int B, int D, int W, int silu, void* stream);
 long nnz_selective_scan_prompt_workspace_bytes(int B, int L, int D, int H, int G, int N);
 int nnz_selective_scan_prompt(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
-                              const long* strides, const float* A, int A_per_state, const float* D_skip, const float* dt_bias,
+                              const long* strides, const float* A, int A_form, const float* D_skip, const float* dt_bias,
                               int softplus, float* state, long state_batch_stride, void* y, const void* lengths,
                               int lengths_are_int64, void* workspace, long workspace_bytes, int B, int L, int D, int H, int G,
                               int N, void* stream);
 int nnz_selective_scan_token(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
-                             const long* strides, const float* A, int A_per_state, const float* D_skip, const float* dt_bias,
+                             const long* strides, const float* A, int A_form, const float* D_skip, const float* dt_bias,
                              int softplus, float* state, long state_batch_stride, void* y, const void* active, int B, int D,
                              int H, int G, int N, void* stream);
 

@@ -220,7 +220,7 @@ struct ScanStateArgs {
   const void* Bm;        // [B][L][G][N], strides bb, bt, bg, 1
   const void* Cm;        // strides cb, ct, cg, 1
   const void* z;         // [B][L][D], strides zb, zt, 1, or null
-  const float* A;        // [H][N] (a_n = 1) or [H] (a_n = 0)
+  const float* A;        // [H][N] (a_n = 1) or [H] (a_n = 0); with a_log its entries are log(-A)
   const float* Dv;       // [H] or null
   const float* dt_bias;  // [H] or null
   float* state;          // [B][D][N], batch stride sb, rows contiguous; or null (zeros, nothing kept)
@@ -229,7 +229,7 @@ struct ScanStateArgs {
   float* part_h;         // [chunks][B][D][N]: end state of chunk c from a zero entry, then (scan_join_kernel) the true entry state of c
   float* part_d;         // [chunks][B][D]: sum of D_t over chunk c
   long xb, xt, db, dtt, bb, bt, bg, cb, ct, cg, zb, zt, sb;
-  int B, L, D, H, G, softplus, len64, a_n;
+  int B, L, D, H, G, softplus, len64, a_n, a_log;
   int rep;               // channels of a head
   int dg;                // channels of a group
   int nch, wpg;          // channels of a workgroup, workgroups of a group
@@ -255,8 +255,11 @@ __device__ __forceinline__ float softplus_hw(float x) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-// A in units of log 2; an infinite decay becomes a huge one, so that a padding token's D_t = 0 leaves the state alone
-__device__ __forceinline__ float decay2(float A) {
+// A[head][n] in units of log 2; an infinite decay becomes a huge one, so that a padding token's D_t = 0 leaves the state alone
+template <int N>
+__device__ __forceinline__ float decay2(const ScanStateArgs& a, int head, int n) {
+  float A = a.a_n ? a.A[(long)head * N + n] : a.A[head];
+  if (a.a_log) A = -exp_fine(A > 88.f ? 88.f : A);
   const float v = A * LOG2E;
   return v < -3.0e38f ? -3.0e38f : v;
 }
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
     prow[q] = (((long)chunk * a.B + b) * a.D + md) * N + sub * NS;
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
-      A2[q][n] = decay2(a.a_n ? a.A[(long)mh * N + sub * NS + n] : a.A[mh]);
+      A2[q][n] = decay2<N>(a, mh, sub * NS + n);
       h[q][n] = MODE == 2 ? a.part_h[prow[q] + n] : MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
     }
   }
@@ -521,7 +524,7 @@ __global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
   const long dn = (long)a.D * N, i = (long)blockIdx.x * LN + lane;
   const long at = i < dn ? i : dn - 1;
   const int d = (int)(at / N), hd = d / a.rep;
-  const float A2 = decay2(a.a_n ? a.A[(long)hd * N + at % N] : a.A[hd]);
+  const float A2 = decay2<N>(a, hd, (int)(at % N));
   const int per = (a.chunks + SEG - 1) / SEG;
   const int c0 = seg * per, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
   float* ph = a.part_h + (long)b * dn + at;
@@ -575,7 +578,7 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
   float acc = 0.f;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    const float A2 = decay2(a.a_n ? a.A[(long)head * N + sub * NS + n] : a.A[head]);
+    const float A2 = decay2<N>(a, head, sub * NS + n);
     const float h = fmaf(__builtin_amdgcn_exp2f(dl * A2), st[n], u * (float)bp[n]);
     st[n] = h;
     acc = fmaf(h, (float)cp[n], acc);
@@ -713,7 +716,7 @@ extern "C" long nnz_selective_scan_prompt_workspace_bytes(int B, int L, int D, i
 }
 
 extern "C" int nnz_selective_scan_prompt(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
-                                         const long* strides, const float* A, int A_per_state, const float* D_skip,
+                                         const long* strides, const float* A, int A_form, const float* D_skip,
                                          const float* dt_bias, int softplus, float* state, long state_batch_stride, void* y,
                                          const void* lengths, int lengths_are_int64, void* workspace, long workspace_bytes,
                                          int B, int L, int D, int H, int G, int N, void* stream) {
@@ -722,7 +725,7 @@ extern "C" int nnz_selective_scan_prompt(const void* x, const void* dt, const vo
   const ScanSplit sp = scan_split(B, L, D, G);
   if (sp.chunks > 1 && (!workspace || workspace_bytes < (long)sp.chunks * B * D * (N + 1) * 4)) return NNZ_EINVAL;
   ScanStateArgs a = {};
-  a.x = x; a.dt = dt; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.a_n = A_per_state; a.Dv = D_skip; a.dt_bias = dt_bias;
+  a.x = x; a.dt = dt; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.a_n = A_form & 1; a.a_log = A_form >> 1 & 1; a.Dv = D_skip; a.dt_bias = dt_bias;
   a.state = state; a.sb = state_batch_stride; a.y = y; a.len = lengths; a.len64 = lengths_are_int64;
   a.xb = strides[0]; a.xt = strides[1]; a.db = strides[2]; a.dtt = strides[3]; a.bb = strides[4]; a.bt = strides[5];
   a.bg = strides[6]; a.cb = strides[7]; a.ct = strides[8]; a.cg = strides[9]; a.zb = strides[10]; a.zt = strides[11];
@@ -737,13 +740,13 @@ extern "C" int nnz_selective_scan_prompt(const void* x, const void* dt, const vo
 }
 
 extern "C" int nnz_selective_scan_token(const void* x, const void* dt, const void* Bm, const void* Cm, const void* z, int type,
-                                        const long* strides, const float* A, int A_per_state, const float* D_skip,
+                                        const long* strides, const float* A, int A_form, const float* D_skip,
                                         const float* dt_bias, int softplus, float* state, long state_batch_stride, void* y,
                                         const void* active, int B, int D, int H, int G, int N, void* stream) {
   using namespace nnz;
   if (!x || !dt || !Bm || !Cm || !A || !y || !state || !strides || !scan_shape_ok(B, 1, D, H, G, N)) return NNZ_EINVAL;
   ScanStateArgs a = {};
-  a.x = x; a.dt = dt; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.a_n = A_per_state; a.Dv = D_skip; a.dt_bias = dt_bias;
+  a.x = x; a.dt = dt; a.Bm = Bm; a.Cm = Cm; a.z = z; a.A = A; a.a_n = A_form & 1; a.a_log = A_form >> 1 & 1; a.Dv = D_skip; a.dt_bias = dt_bias;
   a.state = state; a.sb = state_batch_stride; a.y = y; a.len = active;
   a.xb = strides[0]; a.db = strides[1]; a.bb = strides[2]; a.bg = strides[3]; a.cb = strides[4]; a.cg = strides[5];
   a.zb = strides[6];

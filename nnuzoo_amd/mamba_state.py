@@ -5,8 +5,8 @@ the projections around them write and read them.
 
   causal_conv1d_prompt(x, weight, bias, activation, conv_state, lengths)                  (B, L, D) -> (B, L, D)
   causal_conv1d_token(x, conv_state, weight, bias, activation, active)                    (B, D) -> (B, D)
-  selective_scan_prompt(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths)       (B, L, D) -> (B, L, D)
-  selective_scan_token(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, active)         (B, D) -> (B, D)
+  selective_scan_prompt(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, ...)  (B, L, D) -> (B, L, D)
+  selective_scan_token(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, active, ...)    (B, D) -> (B, D)
 
 conv_state (B, D, W) holds the last W inputs of every sequence, state (B, D, N) its scan state; both are read and brought up to date
 IN PLACE.  A prompt may continue an earlier one.  lengths (B,): tokens of each sequence in a padded batch; nothing behind them is
@@ -192,9 +192,11 @@ _Long7, _Long12 = ctypes.c_long * 7, ctypes.c_long * 12
 def selective_scan_prompt(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                           D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                           dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False,
-                          state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                          A_is_log: bool = False) -> torch.Tensor:
     """h_t = exp(s_t A) h_{t-1} + s_t x_t B_t, y_t = (<C_t, h_t> + D x_t) * silu(z_t) with s_t = [softplus](dt_t + dt_bias) over the
-    tokens of every sequence; h starts from `state` (zeros without one) and is left there"""
+    tokens of every sequence; h starts from `state` (zeros without one) and is left there.  A_is_log: A holds log(-A), the form in which
+    the blocks keep it"""
     name = "selective_scan_prompt"
     dev = need_device(name, x, dt, A, B, C, D, z, dt_bias, state, lengths)
     x, dt, B, C, z, A, D, dt_bias, d, h, g, n = _scan_checks(name, x, dt, A, B, C, D, z, dt_bias, state, 3)
@@ -207,7 +209,7 @@ def selective_scan_prompt(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
         ws_bytes = load().nnz_selective_scan_prompt_workspace_bytes(batch, L, d, h, g, n)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_selective_scan_prompt", dev, x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(z), ELEM[x.dtype],
-               strides, A.data_ptr(), A.dim() - 1, ptr(D), ptr(dt_bias), int(dt_softplus), ptr(state),
+               strides, A.data_ptr(), A.dim() - 1 + 2 * bool(A_is_log), ptr(D), ptr(dt_bias), int(dt_softplus), ptr(state),
                0 if state is None else state.stride(0), y.data_ptr(), ptr(lengths),
                int(lengths is not None and lengths.dtype == torch.int64), ptr(ws), ws_bytes, batch, L, d, h, g, n)
     return y
@@ -216,7 +218,7 @@ def selective_scan_prompt(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
 def selective_scan_token(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                          D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                          dt_bias: Optional[torch.Tensor] = None, dt_softplus: bool = False, *, state: torch.Tensor,
-                         active: Optional[torch.Tensor] = None) -> torch.Tensor:
+                         active: Optional[torch.Tensor] = None, A_is_log: bool = False) -> torch.Tensor:
     """selective_scan_prompt for one token of every active sequence: x, z (B, D), dt (B, H), B, C (B, G, N) or (B, N)"""
     name = "selective_scan_token"
     dev = need_device(name, x, dt, A, B, C, D, z, dt_bias, state, active)
@@ -227,6 +229,6 @@ def selective_scan_token(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: 
     if y.numel():
         strides = _Long7(x.stride(0), dt.stride(0), *B.stride()[:2], *C.stride()[:2], 0 if z is None else z.stride(0))
         launch("nnz_selective_scan_token", dev, x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(z), ELEM[x.dtype],
-               strides, A.data_ptr(), A.dim() - 1, ptr(D), ptr(dt_bias), int(dt_softplus), state.data_ptr(), state.stride(0),
+               strides, A.data_ptr(), A.dim() - 1 + 2 * bool(A_is_log), ptr(D), ptr(dt_bias), int(dt_softplus), state.data_ptr(), state.stride(0),
                y.data_ptr(), ptr(active), batch, d, h, g, n)
     return y

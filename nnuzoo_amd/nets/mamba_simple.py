@@ -139,8 +139,8 @@ class Mamba(nn.Module):
         dbc = F.linear(u, self.x_proj.weight)
         dt = F.linear(dbc[..., :R], self.dt_proj.weight)
         scan = mamba_state.selective_scan_prompt if prompt else mamba_state.selective_scan_token
-        y = scan(u, dt, -torch.exp(self.A_log.float()), dbc[..., R:R + N], dbc[..., R + N:], self.D, z=xz[..., di:],
-                 dt_bias=self.dt_proj.bias, dt_softplus=True, state=ssm_state, **which)
+        y = scan(u, dt, self.A_log, dbc[..., R:R + N], dbc[..., R + N:], self.D, z=xz[..., di:],
+                 dt_bias=self.dt_proj.bias, dt_softplus=True, state=ssm_state, A_is_log=True, **which)
         return F.linear(y, self.out_proj.weight, self.out_proj.bias)
 
     @torch.no_grad()

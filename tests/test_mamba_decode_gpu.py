@@ -100,6 +100,35 @@ def test_step_leaves_inactive_sequences_alone(hip_lib):
 
 
 @gpu
+@pytest.mark.parametrize("name,make", BLOCKS, ids=[b[0] for b in BLOCKS])
+def test_captured_steps(hip_lib, name, make):
+    """a decoder's step as one graph: every replay moves the states on and gives what the eager step gives"""
+    m, x, _ = make()
+    B, L = x.shape[:2]
+    token = x[:, :1].clone()
+    caches = [m.allocate_inference_cache(B) for _ in range(2)]
+    for conv, ssm in caches:
+        m.prompt(x, conv, ssm)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            m.step(token, *m.allocate_inference_cache(B))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.step(token, *caches[0])[0]
+    for t in range(4):
+        token.copy_(x[:, t % L:t % L + 1])
+        graph.replay()
+        want = m.step(token, *caches[1])[0]
+        torch.cuda.synchronize()
+        _close(out, want.cpu(), 1e-5, f"{name} replay {t}")
+        for a, b in zip(*caches):
+            _close(a, b.cpu(), 1e-5, f"{name} state {t}")
+
+
+@gpu
 def test_decoding_under_autocast(hip_lib):
     """fp16 projections around the operators; the scan state stays fp32.  Against fp32: every activation is rounded to 11 bits a few
     times over, and a rounding of the input of the gate or the decays is at most doubled on its way"""

@@ -187,6 +187,28 @@ def test_scan_one_decay_a_head(hip_lib):
 
 
 @gpu
+@pytest.mark.parametrize("per_head", [False, True])
+def test_decays_by_their_logarithm(hip_lib, per_head):
+    """A_is_log: the decays are -exp of what is passed, formed in fp32 (|A_log| + 4 roundings more, relative)"""
+    from nnuzoo_amd.mamba_state import selective_scan_prompt, selective_scan_token
+    v = _scan_data(2, 37, 24, 6, 1, 16, "f32", seed=5, per_head=per_head)
+    v["A"] = torch.log(-v["A"])
+    c = {k: t.cuda() for k, t in v.items()}
+    y = selective_scan_prompt(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], z=c["z"], dt_bias=c["dt_bias"], dt_softplus=True,
+                              state=c["state"], A_is_log=True)
+    t = selective_scan_token(c["x"][:, 0], c["dt"][:, 0], c["A"], c["B"][:, 0], c["C"][:, 0], c["D"], z=c["z"][:, 0], dt_bias=c["dt_bias"],
+                             dt_softplus=True, state=c["state"], A_is_log=True)
+    slack = 1 + 8 * 2.0 ** -24
+    lo, hi = dict(v, A=-torch.exp(v["A"].double()) * slack), dict(v, A=-torch.exp(v["A"].double()))
+    cat = lambda d: {k: (torch.cat((u, u[:, :1]), 1) if k in ("x", "dt", "B", "C", "z") else u) for k, u in d.items()}  # noqa: E731
+    (ya, ea), (sa, es) = _scan_want(cat(hi), [38] * 2, join=32)
+    (yb, _), (sb, _) = _scan_want(cat(lo), [38] * 2, join=32)
+    # a relative change of the decays by 8 roundings moves the results by their difference, to first order, in either direction
+    close(torch.cat((y, t[:, None]), 1), ya, ea + 2 * (ya - yb).abs() + 2.0 ** -22 * ya.abs().amax(), "y")
+    close(c["state"], sa, es + 2 * (sa - sb).abs() + 2.0 ** -22 * sa.abs().amax(), "state")
+
+
+@gpu
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("d,L,join", [(16, 1000, 128), (40, 517, 128), (7, 300, 128)])
 def test_scan_of_several_chunks_ragged(hip_lib, dt, d, L, join):
