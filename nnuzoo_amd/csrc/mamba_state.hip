@@ -54,12 +54,11 @@ template <class T, int W, int V>
 __global__ __launch_bounds__(256) void conv_prompt_kernel(ConvStateArgs a) {
   const int CV = a.D / V;
   const int chunks = (a.L + a.tt - 1) / a.tt;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long)CV * chunks * a.B) return;
-  const int d = (int)(id % CV) * V;
-  const long rest = id / CV;
-  const int t0 = (int)(rest % chunks) * a.tt;
-  const int b = (int)(rest / chunks);
+  const unsigned id = blockIdx.x * 256 + threadIdx.x;   // a launch has less than 2^32 threads
+  if (id >= (unsigned long)CV * chunks * a.B) return;
+  const unsigned rest = id / CV;
+  const int d = (int)(id - rest * CV) * V;
+  const int b = (int)(rest / chunks), t0 = (int)(rest - (unsigned)b * chunks) * a.tt;
   const int len = seq_len(a.len, a.len64, b, a.L);
   const int t1 = t0 + a.tt < a.L ? t0 + a.tt : a.L;
   const T* x = (const T*)a.x + (long)b * a.xb + d;
@@ -147,9 +146,10 @@ __global__ __launch_bounds__(256) void conv_prompt_kernel(ConvStateArgs a) {
 // One token: a thread per (sequence, channel); 3 us, the smallest launch's time, at the sizes of a decoder's step.
 template <class T, int W>
 __global__ __launch_bounds__(256) void conv_token_kernel(ConvStateArgs a) {
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long)a.B * a.D) return;
-  const int b = (int)(id / a.D), d = (int)(id % a.D);
+  const unsigned id = blockIdx.x * 256 + threadIdx.x;   // B * D < 2^32
+  if (id >= (unsigned long)a.B * a.D) return;
+  const unsigned b = id / (unsigned)a.D;
+  const int d = (int)(id - b * a.D);
   T* y = (T*)a.y;
   if (a.len && !((const unsigned char*)a.len)[b]) {
     y[id] = (T)0.f;
@@ -255,13 +255,19 @@ __device__ __forceinline__ float softplus_hw(float x) {
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-// A[head][n] in units of log 2; an infinite decay becomes a huge one, so that a padding token's D_t = 0 leaves the state alone
-template <int N>
-__device__ __forceinline__ float decay2(const ScanStateArgs& a, int head, int n) {
-  float A = a.a_n ? a.A[(long)head * N + n] : a.A[head];
-  if (a.a_log) A = -exp_fine(A > 88.f ? 88.f : A);
-  const float v = A * LOG2E;
-  return v < -3.0e38f ? -3.0e38f : v;
+// decays of NS states from n on, in units of log 2; an infinite one becomes huge, so that a padding token's D_t = 0 leaves the state
+// alone.  All are loaded before the first is used.
+template <int N, int NS>
+__device__ __forceinline__ void load_decays(const ScanStateArgs& a, int head, int n, float (&A2)[NS]) {
+  const float* p = a.a_n ? a.A + (long)head * N + n : a.A + head;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) A2[i] = p[i * a.a_n];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    if (a.a_log) A2[i] = -exp_fine(A2[i] > 88.f ? 88.f : A2[i]);
+    const float v = A2[i] * LOG2E;
+    A2[i] = v < -3.0e38f ? -3.0e38f : v;
+  }
 }
 // sum over the 4 lanes of a channel (quad_perm: no LDS, unlike a shuffle)
 __device__ __forceinline__ float quad_sum(float v) {
@@ -288,7 +294,7 @@ template <class T, int N, int CPL, int MODE>
 __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
   constexpr int NS = N / 4;
   constexpr int IT = SC_TT * CPL / 8;    // token rows of a thread in the staging passes
-  constexpr int ROWS = SC_TT / IT;       // its distance: NT / (nch / 2)
+  constexpr int ROWS = SC_TT / IT;       // their distance: NT / (nch / 2)
   extern __shared__ __attribute__((aligned(16))) float sc_lds[];
   const int nch = a.nch, np = nch / 2;
   float4* s_du = reinterpret_cast<float4*>(sc_lds);     // [SC_TT][nch / 2]: {D, D x} of two channels
@@ -323,11 +329,9 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
     const int md = g * a.dg + (m_on[q] ? ch0 + mc + q : a.dg - 1), mh = md / a.rep;
     srow[q] = (long)b * a.sb + (long)md * N + sub * NS;
     prow[q] = (((long)chunk * a.B + b) * a.D + md) * N + sub * NS;
+    load_decays<N, NS>(a, mh, sub * NS, A2[q]);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      A2[q][n] = decay2<N>(a, mh, sub * NS + n);
-      h[q][n] = MODE == 2 ? a.part_h[prow[q] + n] : MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
-    }
+    for (int n = 0; n < NS; ++n) h[q][n] = MODE == 2 ? a.part_h[prow[q] + n] : MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
   }
   float dsum[CPL] = {};
   // every access walks its rows by a constant step
@@ -466,7 +470,11 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
         const int tt = st + ROWS * i, t = tile + tt;
         if (t < te && on0) {
           const float2 yy = *reinterpret_cast<const float2*>(s_y + tt * nch + 2 * sp);
-          float v0 = fmaf(D0, xv[i].x, yy.x), v1 = fmaf(D1, xv[i].y, yy.y);
+          float v0 = yy.x, v1 = yy.y;
+          if (a.Dv) {
+            v0 = fmaf(D0, xv[i].x, v0);
+            v1 = fmaf(D1, xv[i].y, v1);
+          }
           if (a.z) {
             v0 *= zv[i].x * sigmoid_hw(zv[i].x);
             v1 *= zv[i].y * sigmoid_hw(zv[i].y);
@@ -524,7 +532,9 @@ __global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
   const long dn = (long)a.D * N, i = (long)blockIdx.x * LN + lane;
   const long at = i < dn ? i : dn - 1;
   const int d = (int)(at / N), hd = d / a.rep;
-  const float A2 = decay2<N>(a, hd, (int)(at % N));
+  float A1[1];
+  load_decays<N, 1>(a, hd, (int)(at % N), A1);
+  const float A2 = A1[0];
   const int per = (a.chunks + SEG - 1) / SEG;
   const int c0 = seg * per, c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
   float* ph = a.part_h + (long)b * dn + at;
@@ -553,15 +563,16 @@ __global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
   }
 }
 
-// One token: 4 lanes a channel, each its N / 4 states in one access.  Bound by HBM (the states in and out): 128 x 1536 x 16: 11.8 us =
-// 2.3 TB/s, of which 3.5 us is what the smallest launch takes.
+// One token: 4 lanes a channel, each its N / 4 states in one access.  Bound by HBM (the states in and out): 128 x 1536 x 16: 9.1 us =
+// 3 TB/s, of which 2.8 us is what the smallest launch takes (11.8 us with 64-bit indices and loads behind branches).
 template <class T, int N>
 __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
   constexpr int NS = N / 4;
-  const long id = ((long)blockIdx.x * 256 + threadIdx.x) >> 2;
+  const unsigned id = (blockIdx.x * 256 + threadIdx.x) >> 2;   // 4 B * D < 2^32
   const int sub = threadIdx.x & 3;
-  if (id >= (long)a.B * a.D) return;     // all 4 lanes of a channel leave together
-  const int b = (int)(id / a.D), d = (int)(id % a.D);
+  if (id >= (unsigned long)a.B * a.D) return;     // all 4 lanes of a channel leave together
+  const unsigned b = id / (unsigned)a.D;
+  const int d = (int)(id - b * a.D);
   T* y = (T*)a.y;
   if (a.len && !((const unsigned char*)a.len)[b]) {
     if (sub == 0) y[id] = (T)0.f;
@@ -571,26 +582,36 @@ __global__ __launch_bounds__(256) void scan_token_kernel(ScanStateArgs a) {
   float* st = a.state + (long)b * a.sb + (long)d * N + sub * NS;
   const T* bp = (const T*)a.Bm + (long)b * a.bb + g * a.bg + sub * NS;
   const T* cp = (const T*)a.Cm + (long)b * a.cb + g * a.cg + sub * NS;
-  float dl = (float)((const T*)a.dt)[b * a.db + head] + (a.dt_bias ? a.dt_bias[head] : 0.f);
+  // all loads first, of absent inputs from a place that is there: neither stores nor branches stand between them
+  const T* xp = (const T*)a.x + b * a.xb + d;
+  const T* zp = a.z ? (const T*)a.z + b * a.zb + d : xp;
+  const T xr = *xp, zr = *zp, dr = ((const T*)a.dt)[b * a.db + head];
+  const float Dr = a.Dv ? a.Dv[head] : 0.f, br = a.dt_bias ? a.dt_bias[head] : 0.f;
+  float h[NS], A2[NS];
+  T bv[NS], cv[NS];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) h[n] = st[n];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) bv[n] = bp[n];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) cv[n] = cp[n];
+  load_decays<N, NS>(a, head, sub * NS, A2);
+  const float x = (float)xr, z = (float)zr;
+  float dl = (float)dr + br;
   if (a.softplus) dl = softplus_hw(dl);
-  const float x = (float)((const T*)a.x)[b * a.xb + d];
   const float u = dl * x;
   float acc = 0.f;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    const float A2 = decay2<N>(a, head, sub * NS + n);
-    const float h = fmaf(__builtin_amdgcn_exp2f(dl * A2), st[n], u * (float)bp[n]);
-    st[n] = h;
-    acc = fmaf(h, (float)cp[n], acc);
+    h[n] = fmaf(__builtin_amdgcn_exp2f(dl * A2[n]), h[n], u * (float)bv[n]);
+    acc = fmaf(h[n], (float)cv[n], acc);
   }
+#pragma unroll
+  for (int n = 0; n < NS; ++n) st[n] = h[n];
   acc = quad_sum(acc);
   if (sub == 0) {
-    float v = a.Dv ? fmaf(a.Dv[head], x, acc) : acc;
-    if (a.z) {
-      const float z = (float)((const T*)a.z)[b * a.zb + d];
-      v *= z * sigmoid_hw(z);
-    }
-    y[id] = (T)v;
+    const float v = a.Dv ? fmaf(Dr, x, acc) : acc;
+    y[id] = (T)(a.z ? v * (z * sigmoid_hw(z)) : v);
   }
 }
 
