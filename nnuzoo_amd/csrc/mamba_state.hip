@@ -226,14 +226,15 @@ struct ScanStateArgs {
   float* state;          // [B][D][N], batch stride sb, rows contiguous; or null (zeros, nothing kept)
   void* y;               // [B][L][D] contiguous
   const void* len;       // as above
-  float* part_h;         // [chunks][B][D][N]: end state of chunk c from a zero entry, then (scan_join_kernel) the true entry state of c
+  float* part_h;         // [chunks][B][D][N]: end state of chunk c from a zero entry, then (scan_join_kernel) the true entry state of
+                         // c; without that kernel the last slot, whose summary nobody needs, keeps the sequence's entry state
   float* part_d;         // [chunks][B][D]: sum of D_t over chunk c
   long xb, xt, db, dtt, bb, bt, bg, cb, ct, cg, zb, zt, sb;
   int B, L, D, H, G, softplus, len64, a_n, a_log;
   int rep;               // channels of a head
   int dg;                // channels of a group
   int nch, wpg;          // channels of a workgroup, workgroups of a group
-  int cl, chunks;        // tokens of a chunk
+  int cl, chunks, joined;  // tokens of a chunk; joined: scan_join_kernel runs between MODE 1 and MODE 2
   int pair, pair_dt;     // x and z / dt: two adjacent channels are one aligned access
 };
 
@@ -286,9 +287,12 @@ __device__ __forceinline__ ElemVec<T, 2> ld_pair(const T* p, bool aligned, int s
 // through LDS.  Bound by the vector unit: per token, channel and state a 2^x (quarter rate), two products and two FMAs - 32 cycles a
 // wave of 64 states, 165 us for one pass at 2 x 262144 x 96, N = 16; measured there (f16): summaries 189 us, joining 21, outputs 261.
 // MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks that run in parallel: MODE 1 leaves
-// every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)),
-// scan_join_kernel turns the summaries into entry states, MODE 2 runs the chunks from those.
+// every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)), and MODE 2 runs
+// the chunks from the entry states that the summaries in front of them make: each workgroup joins up to SC_JOIN - 1 of them by
+// itself, scan_join_kernel more.
 constexpr int SC_TT = 16;   // tokens of a tile
+// chunks from which on a kernel of its own joins them (5 ragged prompts of 16 chunks: 42 us a call with it, 37 without)
+constexpr int SC_JOIN = 32;
 
 template <class T, int N, int CPL, int MODE>
 __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
@@ -331,7 +335,30 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
     prow[q] = (((long)chunk * a.B + b) * a.D + md) * N + sub * NS;
     load_decays<N, NS>(a, mh, sub * NS, A2[q]);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[q][n] = MODE == 2 ? a.part_h[prow[q] + n] : MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
+    for (int n = 0; n < NS; ++n) h[q][n] = MODE == 0 && a.state ? a.state[srow[q] + n] : 0.f;
+    // MODE 2 never reads `state`: the workgroup of the last token may have written it already
+    if (MODE == 2 && t0 < te) {
+      const long step = (long)a.B * a.D * N;
+      const float* own = a.part_h + prow[q];
+      const float* first = a.joined ? own : own + (a.chunks - 1 - chunk) * step;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) h[q][n] = first[n];
+      if (!a.joined) {
+        const float* p = own - chunk * step;
+        const float* pd = a.part_d + (long)b * a.D + md;
+#pragma unroll 4
+        for (int c = 0; c < chunk; ++c) {
+          const float sum = pd[(long)c * a.B * a.D];
+#pragma unroll
+          for (int n = 0; n < NS; ++n) h[q][n] = fmaf(__builtin_amdgcn_exp2f(sum * A2[q][n]), h[q][n], p[c * step + n]);
+        }
+      }
+    }
+    if (MODE == 1 && !a.joined && chunk == 0 && m_on[q]) {
+      float* keep = a.part_h + prow[q] + (long)(a.chunks - 1) * a.B * a.D * N;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) keep[n] = a.state ? a.state[srow[q] + n] : 0.f;
+    }
   }
   float dsum[CPL] = {};
   // every access walks its rows by a constant step
@@ -522,9 +549,9 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
   }
 }
 
-// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  A thread per (channel, state); where there
-// are many chunks SEG threads share them: each joins its own run, then starts again from the runs before it (1 261 chunks of
-// 2 x 96 x 16 states: 21 us with 64 runs, 26 us with 16).
+// chunk summaries -> entry states, in place: E_0 = state, E_{c+1} = exp(A sum_c) E_c + S_c.  SEG threads a (channel, state) share the
+// chunks: each joins its own run, then starts again from the runs before it (1 261 chunks of 2 x 96 x 16 states: 21 us with 64
+// runs, 26 us with 16).
 template <int N, int LN, int SEG>
 __global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
   __shared__ float s_p[SEG][LN], s_h[SEG][LN];
@@ -541,19 +568,17 @@ __global__ __launch_bounds__(LN * SEG) void scan_join_kernel(ScanStateArgs a) {
   const float* pd = a.part_d + (long)b * a.D + d;
   const long hs = (long)a.B * dn, ds = (long)a.B * a.D;
   float e = a.state ? a.state[(long)b * a.sb + at] : 0.f;
-  if constexpr (SEG > 1) {
-    float p = 0.f, h = 0.f;
+  float p = 0.f, h = 0.f;
 #pragma unroll 8
-    for (int c = c0; c < c1; ++c) {
-      const float sum = pd[c * ds];
-      h = fmaf(__builtin_amdgcn_exp2f(sum * A2), h, ph[c * hs]);
-      p += sum;
-    }
-    s_p[seg][lane] = p;
-    s_h[seg][lane] = h;
-    __syncthreads();
-    for (int s = 0; s < seg; ++s) e = fmaf(__builtin_amdgcn_exp2f(s_p[s][lane] * A2), e, s_h[s][lane]);
+  for (int c = c0; c < c1; ++c) {
+    const float sum = pd[c * ds];
+    h = fmaf(__builtin_amdgcn_exp2f(sum * A2), h, ph[c * hs]);
+    p += sum;
   }
+  s_p[seg][lane] = p;
+  s_h[seg][lane] = h;
+  __syncthreads();
+  for (int s = 0; s < seg; ++s) e = fmaf(__builtin_amdgcn_exp2f(s_p[s][lane] * A2), e, s_h[s][lane]);
   if (i >= dn) return;
 #pragma unroll 8
   for (int c = c0; c < c1; ++c) {
@@ -657,12 +682,14 @@ static int scan_prompt_run(const ScanStateArgs& a, hipStream_t s) {
   } else {
     if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 1>, lds1, c1)) != hipSuccess) return (int)e;
     if ((e = ensure_dyn_lds((const void*)scan_prompt_kernel<T, N, CPL, 2>, lds, c2)) != hipSuccess) return (int)e;
-    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), grid, block, lds1, s, a);
+    const dim3 sums(a.G * a.wpg, a.joined ? a.chunks : a.chunks - 1, a.B);
+    NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 1>), sums, block, lds1, s, a);
     NNZ_LAUNCH_CHECK();
-    const long dn = (long)a.D * N;
-    if (a.chunks > 64) NNZ_LAUNCH((scan_join_kernel<N, 16, 64>), dim3((unsigned)((dn + 15) / 16), a.B), dim3(1024), 0, s, a);
-    else NNZ_LAUNCH((scan_join_kernel<N, 64, 1>), dim3((unsigned)((dn + 63) / 64), a.B), dim3(64), 0, s, a);
-    NNZ_LAUNCH_CHECK();
+    if (a.joined) {
+      const long dn = (long)a.D * N;
+      NNZ_LAUNCH((scan_join_kernel<N, 16, 64>), dim3((unsigned)((dn + 15) / 16), a.B), dim3(1024), 0, s, a);
+      NNZ_LAUNCH_CHECK();
+    }
     NNZ_LAUNCH((scan_prompt_kernel<T, N, CPL, 2>), grid, block, lds, s, a);
   }
   NNZ_LAUNCH_CHECK();
@@ -754,6 +781,7 @@ extern "C" int nnz_selective_scan_prompt(const void* x, const void* dt, const vo
   a.part_d = a.part_h + (long)sp.chunks * B * D * N;
   a.B = B; a.L = L; a.D = D; a.H = H; a.G = G; a.softplus = softplus;
   a.rep = D / H; a.dg = D / G; a.nch = sp.nch; a.wpg = sp.wpg; a.cl = sp.cl; a.chunks = sp.chunks;
+  a.joined = sp.chunks >= SC_JOIN;
   const uintptr_t m = 2 * (uintptr_t)elem_size(type) - 1;   // a pair's alignment; a group begins at an even channel
   a.pair = (((uintptr_t)x | (uintptr_t)z | (uintptr_t)y) & m) == 0 && ((a.xb | a.xt | a.zb | a.zt | D | a.dg) & 1) == 0;
   a.pair_dt = a.rep == 1 && ((uintptr_t)dt & m) == 0 && ((a.db | a.dtt | a.dg) & 1) == 0;
