@@ -285,7 +285,7 @@ __device__ __forceinline__ ElemVec<T, 2> ld_pair(const T* p, bool aligned, int s
 // 4 lanes share CPL channels and hold N / 4 states of each; a workgroup has nch = 16 CPL channels a wave of one group and walks
 // its tokens in tiles: every (token, channel) of a tile is loaded and turned into D_t, D_t x_t once, B and C are widened once, all
 // through LDS.  Bound by the vector unit: per token, channel and state a 2^x (quarter rate), two products and two FMAs - 32 cycles a
-// wave of 64 states, 165 us for one pass at 2 x 262144 x 96, N = 16; measured there (f16): summaries 189 us, joining 21, outputs 261.
+// wave of 64 states, 165 us for one pass at 2 x 262144 x 96, N = 16; measured there (f16): summaries 200 us, joining 21, outputs 270.
 // MODE 0: whole sequences in one launch.  Long sequences of few channels are cut into chunks that run in parallel: MODE 1 leaves
 // every chunk's summary (end state from a zero entry, sum of D_t: a chunk multiplies its entry state by exp(A sum D)), and MODE 2 runs
 // the chunks from the entry states that the summaries in front of them make: each workgroup joins up to SC_JOIN - 1 of them by
