@@ -180,3 +180,75 @@ def selective_scan(x, dt, A, Bm, C, D, z, dt_bias, softplus, state, lengths, joi
             else:
                 y[i, t], e[i, t] = s, es
     return (y, e), (h, eh)
+
+
+def causal_conv_rows(x, w, b, silu, state, lengths):
+    """causal_conv for all sequences and tokens at once; the same values and bounds"""
+    x, w = x.double().cpu(), w.double().cpu()
+    B, L, D = x.shape
+    W = w.shape[1]
+    b = torch.zeros(D, dtype=torch.float64) if b is None else b.double().cpu()
+    state = torch.zeros(B, D, W, dtype=torch.float64) if state is None else state.double().cpu()
+    seen = torch.cat((state.transpose(1, 2), x), 1)                     # token t lies at W + t
+    s, size = b.expand(B, L, D).clone(), b.abs().expand(B, L, D).clone()
+    for j in range(W):
+        term = w[:, j] * seen[:, 1 + j:1 + j + L]
+        s += term
+        size += term.abs()
+    es = (W + 1) * U * size
+    y, e = _silu(s, es) if silu else (s, es)
+    n = torch.as_tensor(lengths)
+    there = (torch.arange(L) < n[:, None])[..., None]
+    at = (n[:, None] + torch.arange(W))[..., None].expand(B, W, D)
+    zero = torch.zeros((), dtype=torch.float64)
+    return (torch.where(there, y, zero), torch.where(there, e, zero)), seen.gather(1, at).transpose(1, 2)
+
+
+def selective_scan_rows(x, dt, A, Bm, C, D, z, dt_bias, softplus, state, lengths, join=0):
+    """selective_scan for all sequences at once.  `join`: tokens of the chunks that a fast implementation cuts the sequences into: the
+    state behind a chunk is exp(A sum of D_t) entry + the chunk's own, so that beside the recurrence's roundings the sum of `join` time
+    steps counts, (join - 1) U of itself, through the exponential (A sum D exp(A sum D) entry), and the roundings of the joining
+    itself: |A sum D| 4 U + 2 U of the exponential, one of the FMA"""
+    x, dt, Bm, C = (t.double().cpu() for t in (x, dt, Bm, C))
+    B, L, d = x.shape
+    H, (G, N) = dt.shape[-1], Bm.shape[-2:]
+    A = A.double().cpu()
+    A = (A[:, None].expand(H, N) if A.dim() == 1 else A).repeat_interleave(d // H, 0)
+    per = lambda t: torch.zeros(d, dtype=torch.float64) if t is None else t.double().cpu().repeat_interleave(d // H)  # noqa: E731
+    Dv, bias = per(D), per(dt_bias)
+    h = torch.zeros(B, d, N, dtype=torch.float64) if state is None else state.double().cpu().clone()
+    z = None if z is None else z.double().cpu()
+    eh = torch.zeros_like(h)
+    y, e = torch.zeros_like(x), torch.zeros_like(x)
+    n = torch.as_tensor(lengths)
+    entry, steps = h, torch.zeros(B, d, dtype=torch.float64)            # at the chunk's first token; sum of its time steps
+    for t in range(int(n.max())):
+        on = n > t
+        o2, o3 = on[:, None], on[:, None, None]
+        raw = dt[:, t].repeat_interleave(d // H, -1) + bias
+        dl = torch.nn.functional.softplus(raw, threshold=1e9) if softplus else raw
+        e_raw = U * raw.abs()
+        e_dl = (e_raw * raw.sigmoid() + 8 * U * dl.abs()) if softplus else e_raw
+        dA = dl[..., None] * A
+        a = torch.exp(dA)
+        e_a = a * (dA.abs() * 4 * U + A.abs() * e_dl[..., None] + 2 * U)
+        bb, cc = Bm[:, t].repeat_interleave(d // G, 1), C[:, t].repeat_interleave(d // G, 1)
+        u = dl * x[:, t]
+        e_u = e_dl * x[:, t].abs() + U * u.abs()
+        term = u[..., None] * bb
+        new = a * h + term
+        e_new = a * eh + e_a * (h.abs() + eh) + e_u[..., None] * bb.abs() + 3 * U * ((a * h).abs() + term.abs())
+        steps = steps + dl
+        if join and (t + 1) % join == 0:
+            sA = (steps[..., None] * A).abs()
+            kept = torch.exp(steps[..., None] * A) * entry.abs()
+            e_new = e_new + kept * (sA * (join + 3) * U + 2 * U) + U * new.abs()
+            entry, steps = new, torch.zeros_like(steps)
+        h, eh = torch.where(o3, new, h), torch.where(o3, e_new, eh)
+        s = (new * cc).sum(-1) + Dv * x[:, t]
+        es = (e_new * cc.abs()).sum(-1) + (N + 3) * U * ((new * cc).abs().sum(-1) + (Dv * x[:, t]).abs())
+        if z is not None:
+            g, eg = _silu(z[:, t], torch.zeros_like(z[:, t]))
+            s, es = s * g, es * g.abs() + s.abs() * eg + 2 * U * (s * g).abs()
+        y[:, t], e[:, t] = torch.where(o2, s, torch.zeros_like(s)), torch.where(o2, es, torch.zeros_like(es))
+    return (y, e), (h, eh)
