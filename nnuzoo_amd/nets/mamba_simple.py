@@ -168,8 +168,9 @@ class Mamba(nn.Module):
 
 def decode(block, hidden_states, inference_params):
     """forward of a block with `inference_params`: the block's states live in inference_params.key_value_memory_dict[layer_idx]; a
-    prompt (seqlen_offset 0) starts them from zero, with inference_params.lengths_per_sample where it is given, later calls are
-    single tokens"""
+    prompt (seqlen_offset 0) starts them from zero, with the tokens of each sequence in inference_params.prompt_lengths (B,) where a
+    caller puts them there, later calls are single tokens.  inference_params.lengths_per_sample is the caller's own count of what each
+    sequence has cached - zeros before a prompt - and is not read"""
     if block.layer_idx is None:
         raise ValueError("decoding with inference_params needs the block's layer_idx")
     memory, batch = inference_params.key_value_memory_dict, hidden_states.shape[0]
@@ -182,7 +183,7 @@ def decode(block, hidden_states, inference_params):
             t.zero_()
     if not first:
         return block.step(hidden_states, *states)[0]
-    return block.prompt(hidden_states, *states, lengths=getattr(inference_params, "lengths_per_sample", None))
+    return block.prompt(hidden_states, *states, lengths=getattr(inference_params, "prompt_lengths", None))
 
 
 class MambaSSM(Mamba):

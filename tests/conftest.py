@@ -65,6 +65,14 @@ _TIER_BY_NAME = {
 }
 
 
+# Tests that hold a wrong value: run as they are, and expected to fail.
+_WRONG_VALUE = {
+    "test_inference_params_and_ragged_prompts":
+        "hands prompt lengths over in lengths_per_sample, which counts the tokens that each sequence has cached and is 0 before a "
+        "prompt (test_mamba_decode_calls_gpu.py has its other checks, with prompt_lengths)",
+}
+
+
 def collection_tier(item) -> int:
     name = item.name.split("[")[0]
     if name in _TIER_BY_NAME:
@@ -74,3 +82,6 @@ def collection_tier(item) -> int:
 
 def pytest_collection_modifyitems(config, items):
     items.sort(key=collection_tier)          # stable: keeps the order inside a tier
+    for item in items:
+        if item.name.split("[")[0] in _WRONG_VALUE:
+            item.add_marker(pytest.mark.xfail(reason=_WRONG_VALUE[item.name.split("[")[0]], strict=True))
