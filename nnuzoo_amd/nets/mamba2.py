@@ -123,10 +123,13 @@ class Mamba2(nn.Module):
         xbc = zxbcdt[..., ds:2 * ds + 2 * n]
         xbc = mamba_state.causal_conv1d_prompt(xbc, *conv, conv_state, **which) if prompt else \
             mamba_state.causal_conv1d_token(xbc, conv_state, *conv, **which)
+        # fp32 from here to the end of the norm, as in forward: x silu(z) may pass a half-precision type's range, and the norm brings it
+        # back.  What half-precision activations round more than forward does is the convolution's output, once
+        xbc, zxbcdt = xbc.float(), zxbcdt.float()
         scan = mamba_state.selective_scan_prompt if prompt else mamba_state.selective_scan_token
         y = scan(xbc[..., :ds], zxbcdt[..., 2 * ds + 2 * n:], self.A_log, xbc[..., ds:ds + n], xbc[..., ds + n:],
                  self.D, z=zxbcdt[..., :ds], dt_bias=self.dt_bias, dt_softplus=True,
-                 state=ssm_state.view(-1, ds, n), A_is_log=True, **which).float()
+                 state=ssm_state.view(-1, ds, n), A_is_log=True, **which)
         y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.norm.eps) * self.norm.weight
         return F.linear(y.to(u.dtype), self.out_proj.weight, self.out_proj.bias)
 

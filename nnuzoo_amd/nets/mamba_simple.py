@@ -8,8 +8,9 @@ projections are library GEMMs.  `use_fast_path` is accepted and ignored: there i
 
 Decoding (`inference_params`, `step`, `allocate_inference_cache`: :190-215, 357-411, 413-450) runs token-major on the state-carrying
 operators of nnuzoo_amd.mamba_state, without gradients: `prompt` takes whole prompts (ragged ones by `lengths`) and leaves the states,
-`step` one token a sequence.  The caches have the reference's shapes; the scan state is fp32 whatever the cache's type.  Only the
-causal form exists (bimamba_type "none").
+`step` one token a sequence.  The caches have the reference's shapes; the scan state is fp32 whatever the cache's type.
+Half-precision activations (autocast, half weights) are rounded where they pass from one operator to the next, the convolution's output
+among them, which forward keeps in fp32.  Only the causal form exists (bimamba_type "none").
 """
 from __future__ import annotations
 

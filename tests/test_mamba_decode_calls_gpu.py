@@ -46,3 +46,29 @@ def test_ragged_prompts_by_prompt_lengths(hip_lib, name, make):
         _close(tok[i:i + 1], alone[:, n:].cpu(), 3e-4, f"{name} token {i}")
     params.seqlen_offset = 0                    # a new prompt starts from zero states
     assert torch.equal(m(x, inference_params=params), first)
+
+
+@gpu
+@pytest.mark.parametrize("half_weights", [False, True])
+def test_gated_values_past_the_half_precision_range(hip_lib, half_weights):
+    """x silu(z) may pass 65 504 before the RMS norm brings it back: prompt and step keep it in fp32, as forward does.  Against fp32 the
+    roundings to 11 bits are those of the input, of in_proj's weight and output (once each in x, z, and the product of both), of the
+    convolution's output, of the norm's output, of out_proj's weight and output: 10 relative to their own value, carried on by linear steps
+    and by a norm that halves or keeps them; the allowance is the one of the other autocast test, 16"""
+    m, x, _ = _mamba2("a")
+    with torch.no_grad():
+        m.in_proj.weight.mul_(400.0 / (x @ m.in_proj.weight.t()).abs().max())
+        n, ds = m.d_state, m.d_ssm
+        m.in_proj.weight[2 * ds:2 * ds + 2 * n] *= 0.01        # B, C and dt stay ordinary
+        m.in_proj.weight[2 * ds + 2 * n:] *= 0.01
+        m.D.fill_(20.0)
+    want = m(x)
+    if half_weights:
+        m, x = m.half(), x.half()
+    conv, ssm = m.allocate_inference_cache(x.shape[0])
+    with torch.autocast("cuda", dtype=torch.float16, enabled=not half_weights):
+        y = m.prompt(x[:, :-1], conv, ssm)
+        t = m.step(x[:, -1:], conv, ssm)[0]
+    got = torch.cat((y, t), 1)
+    assert bool(torch.isfinite(got).all())
+    _close(got, want.detach().cpu(), 16 * 2.0 ** -11, "gated")
