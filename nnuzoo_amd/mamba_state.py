@@ -19,13 +19,14 @@ N: 4, 8, 16 or 32.  Activations fp32, fp16 or bf16, all of one type; parameters 
 activations' type or fp32).
 
 These operators have no backward (training: nnuzoo_amd.mamba_block, nnuzoo_amd.selective_scan): an input that requires a gradient
-is refused while gradients are being recorded.  There is no CPU path."""
+is refused while gradients are being recorded, one that carries a forward-mode tangent always.  There is no CPU path."""
 from __future__ import annotations
 
 import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import load, ptr
 from .launch import ELEM, launch, need_device, need_elem
@@ -35,6 +36,10 @@ STATE_WIDTHS = (4, 8, 16, 32)
 
 
 def _no_grad(name, *tensors):
+    if forward_ad._current_level >= 0:      # within a dual level, which no_grad() does not end
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative")
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
