@@ -265,7 +265,8 @@ __device__ __forceinline__ void load_decays(const ScanStateArgs& a, int head, in
   for (int i = 0; i < NS; ++i) A2[i] = p[i * a.a_n];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    if (a.a_log) A2[i] = -exp_fine(A2[i] > 88.f ? 88.f : A2[i]);
+    // exp_fine takes no infinity (its rounding of x log2 e would be inf - inf); exp(-110) is 0; NaN stays
+    if (a.a_log) A2[i] = -exp_fine(A2[i] > 88.f ? 88.f : A2[i] < -110.f ? -110.f : A2[i]);
     const float v = A2[i] * LOG2E;
     A2[i] = v < -3.0e38f ? -3.0e38f : v;
   }
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(256) void scan_prompt_kernel(ScanStateArgs a) {
       if (on1) y0[(long)t * a.D + 1] = (T)0.f;
     }
   }
-  // the chunk that holds the last token leaves the state (chunks read `state` in scan_join_kernel only)
+  // the chunk that holds the last token leaves the state (MODE 2 reads the copies that scan_join_kernel or MODE 1's first chunk made)
   if (a.state && len > t0 && len <= tend) {
 #pragma unroll
     for (int q = 0; q < CPL; ++q)

@@ -38,3 +38,29 @@ def test_forward_mode_derivatives_are_refused(hip_lib, name):
     for transform in (lambda f: torch.func.jvp(f, (v["x"],), (v["x"],)), lambda f: torch.func.vmap(f)(torch.stack((v["x"], v["x"])))):
         with pytest.raises(RuntimeError):
             transform(lambda t: _four(dict(v, x=t))[name]())
+
+
+@gpu
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("L", [1, 40, 300, 2500])
+def test_log_decays_of_minus_infinity_are_decays_of_zero(hip_lib, per_head, L):
+    """A_is_log with log(-A) = -inf: the state is never damped, as with A = 0; NaN stays NaN"""
+    from nnuzoo_amd.mamba_state import selective_scan_prompt, selective_scan_token
+    v = {k: t.cuda() for k, t in _scan_data(2, L, 8, 8, 1, 16, "f32", seed=L, per_head=per_head).items()}
+    v["A"][::2] = 0.0
+    out = []
+    for log in (False, True):
+        st = v["state"].clone()
+        a = torch.log(-v["A"]) if log else -torch.exp(torch.log(-v["A"]))
+        kw = dict(z=v["z"], dt_bias=v["dt_bias"], dt_softplus=True, state=st, A_is_log=log)
+        y = selective_scan_prompt(v["x"], v["dt"], a, v["B"], v["C"], v["D"], **kw)
+        kw["z"] = v["z"][:, 0]
+        t = selective_scan_token(v["x"][:, 0], v["dt"][:, 0], a, v["B"][:, 0], v["C"][:, 0], v["D"], **kw)
+        out.append((y[:, :, ::2], t[:, ::2], st[:, ::2]))
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
+    a = torch.log(-v["A"])
+    a[1] = float("nan")
+    st = v["state"].clone()
+    y = selective_scan_prompt(v["x"], v["dt"], a, v["B"], v["C"], v["D"], dt_bias=v["dt_bias"], dt_softplus=True, state=st, A_is_log=True)
+    assert bool(torch.isnan(y[:, :, 1]).all()) and bool(torch.isfinite(y[:, :, ::2]).all())
