@@ -776,7 +776,8 @@ int nnz_dropout_backward(const void* dy, int dy_type, void* dx, int dx_type, lon
 /* ---- the state-carrying operators of the 1-D Mamba blocks, token-major (Mamba.step and inference_params,
  * nets/seg_mamba/mamba_simple.py:190-215, 357-411).  type: element type of the activations.  conv_state [B][D][W] (any strides,
  * element type state_type; NULL in the prompt form: zeros, nothing kept) and state [B][D][N] fp32 (contiguous within a sequence)
- * are updated in place.  A_form: 1 for A [H][N], 0 for A [H], + 2 where the entries are log(-A).  lengths: [B] int32 / int64 or NULL; active: [B] bytes or NULL.  W <= 8; N 4, 8, 16, 32.
+ * are updated in place.  A_form: 1 for A [H][N], 0 for A [H], + 2 where the entries are log(-A).  lengths: [B] int32 / int64 or
+ * NULL; active: [B] bytes or NULL.  W <= 8; N 4, 8, 16, 32.  selective_scan_prompt: B <= 65535.
  * strides (host table, elements): prompt {x batch, x token, dt batch, dt token, B batch, B token, B group, C batch, C token,
  * C group, z batch, z token}; token {x batch, dt batch, B batch, B group, C batch, C group, z batch}. */
 int nnz_causal_conv1d_prompt(const void* x, int type, long x_batch_stride, long x_token_stride, const float* weight,

@@ -15,8 +15,8 @@ sequences that take part in a token step; the others keep their states and get 0
 
 Heads: dt is (B, L, H) with D = H * P channels, head by head; A is (H, N) or, one decay a head, (H,); D and dt_bias are (H,).
 B and C are (B, L, G, N), or (B, L, N) for one group; group g serves the channels g * D / G ...  H = D is Mamba, A (H,) is Mamba2.
-N: 4, 8, 16 or 32.  Activations fp32, fp16 or bf16, all of one type; parameters are taken in fp32, states are fp32 (conv_state: the
-activations' type or fp32).
+N: 4, 8, 16 or 32; W: up to 8; the scan over prompts takes at most 65535 sequences a call.  Activations fp32, fp16 or bf16, all of one
+type; parameters are taken in fp32, states are fp32 (conv_state: the activations' type or fp32).
 
 These operators have no backward (training: nnuzoo_amd.mamba_block, nnuzoo_amd.selective_scan): an input that requires a gradient
 is refused while gradients are being recorded, one that carries a forward-mode tangent always.  There is no CPU path."""
@@ -33,6 +33,7 @@ from .launch import ELEM, launch, need_device, need_elem
 
 MAX_WIDTH = 8
 STATE_WIDTHS = (4, 8, 16, 32)
+MAX_PROMPTS = 65535         # sequences of a scan over prompts: the rows of a launch's grid
 
 
 def _no_grad(name, *tensors):
@@ -206,6 +207,8 @@ def selective_scan_prompt(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     dev = need_device(name, x, dt, A, B, C, D, z, dt_bias, state, lengths)
     x, dt, B, C, z, A, D, dt_bias, d, h, g, n = _scan_checks(name, x, dt, A, B, C, D, z, dt_bias, state, 3)
     batch, L = x.shape[:2]
+    if batch > MAX_PROMPTS:
+        raise NotImplementedError(f"{name}: at most {MAX_PROMPTS} sequences a call, got {batch}")
     lengths = _which(name, "lengths", lengths, batch, (torch.int32, torch.int64))
     y = torch.empty((batch, L, d), dtype=x.dtype, device=dev)
     if y.numel():

@@ -64,3 +64,14 @@ def test_log_decays_of_minus_infinity_are_decays_of_zero(hip_lib, per_head, L):
     st = v["state"].clone()
     y = selective_scan_prompt(v["x"], v["dt"], a, v["B"], v["C"], v["D"], dt_bias=v["dt_bias"], dt_softplus=True, state=st, A_is_log=True)
     assert bool(torch.isnan(y[:, :, 1]).all()) and bool(torch.isfinite(y[:, :, ::2]).all())
+
+
+@gpu
+def test_sequences_past_a_grid_are_refused_by_name(hip_lib):
+    from nnuzoo_amd.mamba_state import selective_scan_prompt, selective_scan_token
+    z = lambda *s: torch.zeros(s, device="cuda")  # noqa: E731
+    B = 65536
+    with pytest.raises(NotImplementedError, match="65535 sequences"):
+        selective_scan_prompt(z(B, 2, 4), z(B, 2, 4), z(4, 4), z(B, 2, 4), z(B, 2, 4))
+    assert selective_scan_prompt(z(B - 1, 2, 4), z(B - 1, 2, 4), z(4, 4), z(B - 1, 2, 4), z(B - 1, 2, 4)).shape == (B - 1, 2, 4)
+    assert selective_scan_token(z(B, 4), z(B, 4), z(4, 4), z(B, 4), z(B, 4), state=z(B, 4, 4)).shape == (B, 4)
