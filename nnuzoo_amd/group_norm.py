@@ -150,13 +150,16 @@ def _hooked(m: nn.Module) -> bool:
     return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
 
 
+_hooks_of_all = nn.modules.module._has_any_global_hook      # register_module_forward_hook and its kin
+
+
 def norm_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """act(norm(x)): the operator where `norm` is an nn.GroupNorm, `act` one of its activations and x a device tensor whose channels
     lie innermost (what the token-major mixers of the LightMUNet family hand on; the spatial axes may lie in any order); the two
     modules one after the other otherwise."""
     name = {nn.ReLU: "relu", nn.SiLU: "silu", nn.LeakyReLU: "leaky_relu", nn.Identity: "none"}.get(type(act))
     if (type(norm) is nn.GroupNorm and name is not None and x.is_cuda and x.dtype in ELEM and norm.num_channels <= MAX_CHANNELS
-            and not _hooked(norm) and not _hooked(act)):
+            and not _hooked(norm) and not _hooked(act) and not _hooks_of_all()):
         perm = _token_order(x)
         if perm is not None:
             from . import backends
