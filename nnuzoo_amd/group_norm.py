@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from ._lib import load, ptr
 from .launch import ELEM, first_order, launch, need_device, need_elem
@@ -153,13 +154,21 @@ def _hooked(m: nn.Module) -> bool:
 _hooks_of_all = nn.modules.module._has_any_global_hook      # register_module_forward_hook and its kin
 
 
+def _transformed(*tensors) -> bool:
+    """whether torch.func transforms (vmap, jvp, ..) or forward-mode tangents are at work, which the operator has no rules for"""
+    if torch._C._are_functorch_transforms_active():
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def norm_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
     """act(norm(x)): the operator where `norm` is an nn.GroupNorm, `act` one of its activations and x a device tensor whose channels
     lie innermost (what the token-major mixers of the LightMUNet family hand on; the spatial axes may lie in any order); the two
     modules one after the other otherwise."""
     name = {nn.ReLU: "relu", nn.SiLU: "silu", nn.LeakyReLU: "leaky_relu", nn.Identity: "none"}.get(type(act))
     if (type(norm) is nn.GroupNorm and name is not None and x.is_cuda and x.dtype in ELEM and norm.num_channels <= MAX_CHANNELS
-            and not _hooked(norm) and not _hooked(act) and not _hooks_of_all()):
+            and not _hooked(norm) and not _hooked(act) and not _hooks_of_all()
+            and not _transformed(x, norm.weight, norm.bias)):
         perm = _token_order(x)
         if perm is not None:
             from . import backends

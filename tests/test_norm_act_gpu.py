@@ -29,3 +29,30 @@ def test_hooks_of_all_modules(hip_lib, register):
     finally:
         handle.remove()
     assert sorted(seen) == ["GroupNorm", "SiLU"]
+
+
+@gpu
+@pytest.mark.parametrize("act", ACTS, ids=lambda a: type(a).__name__)
+def test_forward_mode_and_vmap(hip_lib, act):
+    from nnuzoo_amd.group_norm import norm_act
+    norm, x = _case()
+    v, w = torch.randn_like(x), norm.weight.detach()
+
+    def with_weight(f):
+        class Both(nn.Module):
+            def __init__(self):
+                super().__init__()
+                self.norm = norm
+
+            def forward(self, t):
+                return f(t)
+        return lambda u: torch.func.functional_call(Both(), {"norm.weight": u}, (x,))
+    ours, mods = (lambda t: norm_act(norm, act, t)), (lambda t: act(norm(t)))
+    for f, g, at, d in ((ours, mods, x, v), (with_weight(ours), with_weight(mods), w, torch.ones_like(w))):
+        for a, b in zip(torch.func.jvp(f, (at,), (d,)), torch.func.jvp(g, (at,), (d,))):
+            assert torch.equal(a, b)
+        many = torch.stack((at, d))
+        assert torch.equal(torch.func.vmap(f)(many), torch.func.vmap(g)(many))
+    with torch.autograd.forward_ad.dual_level():
+        a, b = (torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(x, v))) for f in (ours, mods))
+        assert torch.equal(a.primal, b.primal) and torch.equal(a.tangent, b.tangent)
