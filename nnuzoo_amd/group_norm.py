@@ -26,7 +26,8 @@ MAX_CHANNELS = 4096     # csrc/group_norm.hip GN_MAX_C
 
 
 def _rows(x: torch.Tensor):
-    """(x or its contiguous copy, batch stride, row stride): rows of C adjacent elements, evenly spaced within a sample"""
+    """(x or its contiguous copy, batch stride, row stride): rows of C adjacent elements, evenly spaced within a sample.  The copy is made
+    in front of the autograd function, so that what the function saves is part of the graph"""
     C = x.shape[-1]
     if x.stride(-1) == 1 or C == 1:
         step = want = None
@@ -45,9 +46,8 @@ def _rows(x: torch.Tensor):
 
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, slope, out_dtype):
+    def forward(ctx, x, xb, xs, weight, bias, groups, eps, act, slope, out_dtype):
         dev = x.device
-        x, xb, xs = _rows(x)
         y = torch.empty(x.shape, dtype=out_dtype, device=dev)
         N, C = x.shape[0], x.shape[-1]
         stats = None
@@ -74,7 +74,7 @@ class _GroupNormActFn(torch.autograd.Function):
 
 def _backward(ctx, dy):
     x, weight, bias = ctx.saved_tensors
-    _, need_w, need_b, *_ = ctx.needs_input_grad
+    _, _, _, need_w, need_b, *_ = ctx.needs_input_grad
     dev, C, stats = x.device, x.shape[-1], ctx.stats
     make = torch.zeros if stats is None else torch.empty
     dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
@@ -87,7 +87,7 @@ def _backward(ctx, dy):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
                ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C, groups, act, slope)
-    return dx, dw, db, None, None, None, None, None
+    return dx, None, None, dw, db, None, None, None, None, None
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -113,8 +113,8 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     if bias is not None:
         bias = bias.float().contiguous()
     out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
-    return _GroupNormActFn.apply(x, weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation], float(negative_slope),
-                                 out_dtype)
+    return _GroupNormActFn.apply(*_rows(x), weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation],
+                                 float(negative_slope), out_dtype)
 
 
 class GroupNormAct(nn.GroupNorm):
