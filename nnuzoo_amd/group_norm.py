@@ -9,12 +9,13 @@ gradient.
 
 fp32 / fp16 / bf16 in; the output has the input's type, or fp32 under autocast (group_norm is on autocast's fp32 list).
 Statistics are fp64 sums, everything else is computed in fp32 and rounded once.  Results are bit-identical from run to run.
-There is no second derivative and no CPU path."""
+There is no CPU path and, but for norm_act, which stands for two modules that have one, no second derivative."""
 from __future__ import annotations
 
 from typing import Optional
 
 import torch
+import torch.nn.functional as F
 from torch import nn
 from torch.autograd import forward_ad
 
@@ -46,7 +47,7 @@ def _rows(x: torch.Tensor):
 
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, xb, xs, weight, bias, groups, eps, act, slope, out_dtype):
+    def forward(ctx, x, xb, xs, weight, bias, groups, eps, act, slope, out_dtype, twice):
         dev = x.device
         y = torch.empty(x.shape, dtype=out_dtype, device=dev)
         N, C = x.shape[0], x.shape[-1]
@@ -61,12 +62,15 @@ class _GroupNormActFn(torch.autograd.Function):
             ctx.cfg = (xb, xs, N, S, C, groups, act, slope)
         ctx.save_for_backward(x, weight, bias)
         ctx.stats = stats       # of this node's own making: neither input nor output
+        ctx.twice = (groups, eps, act, slope) if twice else None
         return y
 
     @staticmethod
     def backward(ctx, dy):
         if not torch.is_grad_enabled():
             return _backward(ctx, dy)
+        if ctx.twice:
+            return _recorded_backward(ctx, dy)
         with torch.no_grad():
             grads = _backward(ctx, dy)
         return first_order("group_norm_act", grads, (dy, *ctx.saved_tensors))
@@ -87,13 +91,32 @@ def _backward(ctx, dy):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
                ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C, groups, act, slope)
-    return dx, None, None, dw, db, None, None, None, None, None
+    return dx, None, None, dw, db, None, None, None, None, None, None
+
+
+def _recorded_backward(ctx, dy):
+    """the gradients as functions that can be differentiated again (create_graph=True), from the library's group norm: what a caller
+    of the modules that norm_act stands for gets"""
+    x, weight, bias = ctx.saved_tensors
+    groups, eps, act, slope = ctx.twice
+    z = F.group_norm(x.movedim(-1, 1).float(), groups, weight, bias, eps)
+    y = {0: lambda t: t, 1: F.relu, 2: lambda t: F.leaky_relu(t, slope), 3: F.silu}[act](z).movedim(1, -1).to(dy.dtype)
+    grads = [None] * 11
+    which = [i for i in (0, 3, 4) if ctx.needs_input_grad[i]]
+    ins = {0: x, 3: weight, 4: bias}
+    for i, g in zip(which, torch.autograd.grad(y, [ins[i] for i in which], dy, create_graph=True)):
+        grads[i] = g
+    return tuple(grads)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
                    bias: Optional[torch.Tensor] = None, eps: float = 1e-5, activation: Optional[str] = None,
                    negative_slope: float = 0.01) -> torch.Tensor:
     """activation(group_norm(x)) for x (N, *spatial, C); activation: None / "none", "relu", "leaky_relu", "silu"."""
+    return _group_norm_act(x, num_groups, weight, bias, eps, activation, negative_slope, twice=False)
+
+
+def _group_norm_act(x, num_groups, weight, bias, eps, activation, negative_slope, twice):
     dev = need_device("group_norm_act", x, weight, bias)
     need_elem("group_norm_act", x=x, weight=weight, bias=bias)
     if activation not in ACTIVATIONS:
@@ -114,7 +137,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         bias = bias.float().contiguous()
     out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") else x.dtype
     return _GroupNormActFn.apply(*_rows(x), weight, bias, int(num_groups), float(eps), ACTIVATIONS[activation],
-                                 float(negative_slope), out_dtype)
+                                 float(negative_slope), out_dtype, twice)
 
 
 class GroupNormAct(nn.GroupNorm):
@@ -173,7 +196,7 @@ def norm_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
         if perm is not None:
             from . import backends
             backends.note(norm, "hip", "group norm + activation")
-            y = group_norm_act(x.permute(perm), norm.num_groups, norm.weight, norm.bias, norm.eps, name,
-                               getattr(act, "negative_slope", 0.01))
+            y = _group_norm_act(x.permute(perm), norm.num_groups, norm.weight, norm.bias, norm.eps, name,
+                                getattr(act, "negative_slope", 0.01), twice=True)
             return y.permute([perm.index(d) for d in range(x.dim())])
     return act(norm(x))

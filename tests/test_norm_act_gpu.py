@@ -56,3 +56,28 @@ def test_forward_mode_and_vmap(hip_lib, act):
     with torch.autograd.forward_ad.dual_level():
         a, b = (torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(x, v))) for f in (ours, mods))
         assert torch.equal(a.primal, b.primal) and torch.equal(a.tangent, b.tangent)
+
+
+@gpu
+@pytest.mark.parametrize("act", ACTS, ids=lambda a: type(a).__name__)
+def test_second_derivatives(hip_lib, act):
+    """a gradient penalty through token-major activations: the modules' second derivatives, in x, dy and both parameters.  Both sides are
+    fp32 computations of sums over 120 terms in different orders: 1e-4 of the largest value is 2^10 roundings"""
+    from nnuzoo_amd import backends
+    from nnuzoo_amd.group_norm import norm_act
+    norm, x = _case()
+    dy = torch.randn_like(x).requires_grad_(True)
+    out = []
+    for f in (lambda t: norm_act(norm, act, t), lambda t: act(norm(t))):
+        backends.reset()
+        xr = x.clone().requires_grad_(True)
+        ins = (xr, norm.weight, norm.bias)
+        first = torch.autograd.grad(f(xr), ins, dy, create_graph=True)
+        out.append((first, torch.autograd.grad(sum(g.square().sum() for g in first), (*ins, dy), allow_unused=True),
+                    any(k[2] == "hip" for k in backends.COUNTS)))
+    assert out[0][2] and not out[1][2]          # the operator ran on the one side, the modules on the other
+    for got, want in zip(out[0][:2], out[1][:2]):
+        for a, b in zip(got, want):
+            assert (a is None) == (b is None)
+            if a is not None:
+                assert float((a - b).abs().max()) <= 1e-4 * float(b.abs().max())
