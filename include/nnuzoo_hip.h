@@ -754,7 +754,8 @@ int nnz_layer_norm_backward_partial(const float* x, const float* gamma, const fl
  * nets/lm2net.py:119-121,160-171, light_mamba2net.py:480-482,519-531, LightMUNet.py:105-107,144-156).  x: [N][S][C], batch and row
  * strides in elements, C innermost; y, dy, dx contiguous.  Element types 0: fp32, 1: fp16, 2: bf16; y / dy have x's type or fp32.
  * act 0: none, 1: ReLU, 2: LeakyReLU(slope), 3: SiLU.  stats: [N][G][2] = mean, 1 / sqrt(var + eps), written by the forward and read
- * by the backward.  weight / bias fp32 [C] or NULL; dweight / dbias [C] or NULL.  C <= 4096.  Bit-identical from run to run. */
+ * by the backward.  weight / bias fp32 [C] or NULL; dx, dweight, dbias: NULL where not needed (not all three).  C <= 4096.
+ * Bit-identical from run to run. */
 long nnz_group_norm_act_workspace_bytes(long N, long S, int C, int G, int backward);
 int nnz_group_norm_act_forward(const void* x, int x_type, long x_batch_stride, long x_row_stride, const float* weight,
                                const float* bias, void* y, int y_type, float* stats, void* workspace, long workspace_bytes,

@@ -22,7 +22,7 @@ struct GnArgs {
   const void* dy;     // [N][S][C] contiguous
   const float* w;     // [C] or null (ones)
   const float* b;     // [C] or null (zeros)
-  void* out;          // y or dx, [N][S][C] contiguous
+  void* out;          // y or dx, [N][S][C] contiguous; backward: null where x needs no gradient
   float* stats;       // [N][G][2]: mean, 1 / sqrt(var + eps)
   double* gpart;      // [N][nblk][G][2]
   float* cpart;       // backward: [N][nblk][C][2]: sum dz, sum dz xhat
@@ -504,7 +504,7 @@ __global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a, int K) {
   for (long n = k; n < a.N; n += K) {
     const TI* x = (const TI*)a.x + n * a.xb + c;
     const TO* dy = (const TO*)a.dy + n * a.S * a.C + c;
-    TI* dx = (TI*)a.out + n * a.S * a.C + c;
+    TI* dx = a.out ? (TI*)a.out + n * a.S * a.C + c : nullptr;
     const float mu = a.stats[(n * a.G + g) * 2], rstd = a.stats[(n * a.G + g) * 2 + 1];
     double s = 0.0, t = 0.0;
     if (p.on) {
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(GN_SNT) void gn_small_bwd_kernel(GnArgs a, int K) {
     }
     gn_team_sum<T>(s, t, red);
     const float m1 = (float)(s / m), m2 = (float)(t / m);
-    if (p.on) {
+    if (p.on && a.out) {
 #pragma unroll 2
       for (long r = p.rr; r < a.S; r += p.R) {
         float v[V], d[V];
@@ -650,6 +650,7 @@ static int gn_large_bwd(GnArgs a, hipStream_t s) {
   const long pairs4 = (a.N * a.G + 3) / 4, pair_wgs = pairs4 < GN_MAX_WG ? pairs4 : GN_MAX_WG;
   NNZ_LAUNCH(gn_bwd_finish_kernel, dim3((unsigned)(pair_wgs + (a.C + GN_FC - 1) / GN_FC)), dim3(GN_NT), 0, s, a, pair_wgs);
   NNZ_LAUNCH_CHECK();
+  if (!a.out) return NNZ_OK;
   gn_split(a, V, GN_TARGET_APPLY);
   NNZ_LAUNCH((gn_bwd_apply_kernel<TI, TO, V, GV>), gn_grid(a.N * a.nblk), dim3(GN_NT), 0, s, a);
   NNZ_LAUNCH_CHECK();
@@ -747,7 +748,7 @@ extern "C" int nnz_group_norm_act_backward(const void* x, int x_type, long x_bat
                                            float* dweight, float* dbias, void* workspace, long workspace_bytes, long N, long S,
                                            int C, int G, int act, float slope, void* stream) {
   using namespace nnz;
-  if (!x || !dy || !dx || !stats || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
+  if (!x || !dy || !(dx || dweight || dbias) || !stats || !gn_shape_ok(N, S, C, G) || act < GN_NONE || act > GN_SILU) return NNZ_EINVAL;
   const GnWs w = gn_ws(N, S, C, G, true);
   if (w.bytes && (!workspace || workspace_bytes < w.bytes)) return NNZ_EINVAL;
   GnArgs a = {};

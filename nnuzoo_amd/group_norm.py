@@ -78,10 +78,10 @@ class _GroupNormActFn(torch.autograd.Function):
 
 def _backward(ctx, dy):
     x, weight, bias = ctx.saved_tensors
-    _, _, _, need_w, need_b, *_ = ctx.needs_input_grad
+    need_x, _, _, need_w, need_b, *_ = ctx.needs_input_grad
     dev, C, stats = x.device, x.shape[-1], ctx.stats
     make = torch.zeros if stats is None else torch.empty
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
     dw = make(C, dtype=torch.float32, device=dev) if need_w else None
     db = make(C, dtype=torch.float32, device=dev) if need_b else None
     if stats is not None:
@@ -90,7 +90,7 @@ def _backward(ctx, dy):
         ws_bytes = load().nnz_group_norm_act_workspace_bytes(N, S, C, groups, 1)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
         launch("nnz_group_norm_act_backward", dev, x.data_ptr(), ELEM[x.dtype], xb, xs, dy.data_ptr(), ELEM[dy.dtype],
-               ptr(weight), ptr(bias), stats.data_ptr(), dx.data_ptr(), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C, groups, act, slope)
+               ptr(weight), ptr(bias), stats.data_ptr(), ptr(dx), ptr(dw), ptr(db), ptr(ws), ws_bytes, N, S, C, groups, act, slope)
     return dx, None, None, dw, db, None, None, None, None, None, None
 
 
