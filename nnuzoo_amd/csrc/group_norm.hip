@@ -622,15 +622,22 @@ inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
   return w;
 }
 
-template <class TI, class TO, int V, int GV>
-static int gn_large_fwd(GnArgs a, hipStream_t s) {
+// one function, and so one cache, a kernel: the callers differ in the output's type and the groups of a vector
+template <class TI, int V>
+static int gn_stats(const GnArgs& a, hipStream_t s) {
   static DynLdsCache cache;
-  gn_split(a, V, GN_TARGET);
   const int lds = (GN_NT * V + a.C) * 2 * 8;
   hipError_t e = ensure_dyn_lds((const void*)gn_stats_kernel<TI, V>, lds, cache);
   if (e != hipSuccess) return (int)e;
   NNZ_LAUNCH((gn_stats_kernel<TI, V>), gn_grid(a.N * a.nblk), dim3(GN_NT), lds, s, a);
   NNZ_LAUNCH_CHECK();
+  return NNZ_OK;
+}
+template <class TI, class TO, int V, int GV>
+static int gn_large_fwd(GnArgs a, hipStream_t s) {
+  gn_split(a, V, GN_TARGET);
+  const int rc = gn_stats<TI, V>(a, s);
+  if (rc) return rc;
   NNZ_LAUNCH(gn_stats_finish_kernel, gn_grid(a.N * a.G), dim3(64), 0, s, a);
   NNZ_LAUNCH_CHECK();
   gn_split(a, V, GN_TARGET_APPLY);

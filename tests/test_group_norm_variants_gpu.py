@@ -51,3 +51,16 @@ def test_more_pairs_than_a_launch_has_teams(hip_lib):
         want = oracle(x[part].detach(), 8, w, b, 1e-2, "silu", SLOPE, dy[part])
         close(y[part], *want["y"], "y")
         close(dx[part], *want["dx"], "dx")
+
+
+@gpu
+def test_many_channels_after_a_call_with_few(hip_lib):
+    """4 096 channels take more than 64 KB of LDS; calls of other element types with few channels in between change nothing"""
+    wide = _data(1, 200, 4096, torch.bfloat16, seed=20)
+    few = _data(2, 9000, 32, torch.bfloat16, seed=21)
+    for groups, autocast in ((32, False), (32, True)):
+        _check(*wide[:1], groups, *wide[1:3], wide[3].float() if autocast else wide[3], "none", autocast=autocast)
+        for g in (8, 4):
+            _check(*few[:1], g, *few[1:3], few[3].float(), "none", autocast=True)
+            _check(*few[:1], g, *few[1:3], few[3], "none")
+        _check(*wide[:1], groups, *wide[1:3], wide[3].float() if autocast else wide[3], "none", autocast=autocast)
