@@ -588,15 +588,26 @@ inline void gn_split(GnArgs& a, int V, long target) {
   if (per > most) per = most;
   a.nblk = (int)(per < 1 ? 1 : per);
 }
-// The small-group kernels are taken up to this many elements of a (sample, group).  Up to GN_WAVE of them a wave is team enough once
-// there are more groups than the chip holds workgroups: 100 000 x 4 x 32 in 8 groups, forward and backward: 3.9 ms by workgroups,
-// 0.65 by waves; 3 x 63 x 60 in 6 groups: 14 us by workgroups, 26 by waves.
-constexpr long GN_SMALL = 16384, GN_WAVE = 1024;
-inline bool gn_small(long S, int q) { return q <= GN_SNT && S * q <= GN_SMALL; }
-inline bool gn_by_wave(long N, long S, int G, int q) { return q <= 64 && S * q <= GN_WAVE && N * G > 1024; }
-// teams of a group in the backward: one walks all samples while that is a few passes' work; else as many as fill the chip
+// Which kernels a call takes, by forward + backward on the device, fp32 unless said otherwise (32 channels in 8 groups, other shapes alike):
+// - one launch each way (small groups) up to GN_ROWS rows: 2 x 512 x 32: 20 us against 25 by rows, 2 x 1024: 24 against 26, 2 x 2048: 33
+//   against 26, 2 x 4096: 49 against 26;
+// - and up to GN_SEGS row segments altogether, for a segment narrower than a line costs as much as a line: 16 x 512: 21 against 26, 32 x 512
+//   (2^17): 26 against 26, 32 x 1024: 46 against 27, 128 x 1024: 143 against 37.  From 64 channels a group on a segment is whole lines
+//   (64 x 128 x 512 in 8 groups: 27 against 41);
+// - a wave is team enough for GN_WAVE elements once there are more pairs than workgroups to keep the chip busy: 128 x 128 x 32: 15 us by
+//   waves, 34 by workgroups, 23 by rows; 32 x 32 x 32: 12, 19, 18.  Few pairs of 1 024 elements are quicker by workgroups (32 x 102 x 60 in
+//   6 groups: 13 by workgroups, 20 by waves), so up to 256 pairs half as many elements count.
+constexpr long GN_SMALL = 16384, GN_WAVE = 1024, GN_ROWS = 1024, GN_SEGS = 1L << 17;
+inline bool gn_by_wave(long N, long S, int G, int q) {
+  return q <= 64 && S * q <= (N * G > 256 ? GN_WAVE : GN_WAVE / 2) && N * G > 64;
+}
+inline bool gn_small(long N, long S, int G, int q) {
+  return q <= GN_SNT && S * q <= GN_SMALL && (gn_by_wave(N, S, G, q) || (S <= GN_ROWS && (q >= 64 || N * G * S <= GN_SEGS)));
+}
+// teams of a group in the backward: one walks both samples of two, which spares the launch that adds partial weight gradients; else as
+// many as fill the chip (8 x 512 x 32, forward + backward: 20 us, by one team 36)
 inline int gn_teams(long N, long S, int G, int q) {
-  if (N <= 8 && N * S * q <= 2 * GN_SMALL) return 1;
+  if (N <= 2) return 1;
   long k = (gn_by_wave(N, S, G, q) ? 8192 : 1024) / G;
   if (k > N) k = N;
   return (int)(k < 1 ? 1 : k);
@@ -608,7 +619,7 @@ struct GnWs {
   long gpart, cpart, cc, bytes;
 };
 inline GnWs gn_ws(long N, long S, int C, int G, bool bwd) {
-  if (gn_small(S, C / G)) {
+  if (gn_small(N, S, G, C / G)) {
     const int k = bwd ? gn_teams(N, S, G, C / G) : 1;
     return GnWs{0, 0, 0, k > 1 ? (long)k * C * 8 : 0};
   }
@@ -690,7 +701,7 @@ static int gn_run_small(const GnArgs& a, bool bwd, hipStream_t s) {
 }
 template <class TI, class TO, int V>
 static int gn_run(const GnArgs& a, bool bwd, hipStream_t s) {
-  if (gn_small(a.S, a.q)) {
+  if (gn_small(a.N, a.S, a.G, a.q)) {
     // a vector lies within a group or is one element
     if (V > 1 && a.q % V != 0) return gn_run_small<TI, TO, 1>(a, bwd, s);
     return gn_run_small<TI, TO, V>(a, bwd, s);
