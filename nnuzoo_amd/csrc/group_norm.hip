@@ -604,10 +604,11 @@ inline bool gn_by_wave(long N, long S, int G, int q) {
 inline bool gn_small(long N, long S, int G, int q) {
   return q <= GN_SNT && S * q <= GN_SMALL && (gn_by_wave(N, S, G, q) || (S <= GN_ROWS && (q >= 64 || N * G * S <= GN_SEGS)));
 }
-// teams of a group in the backward: one walks both samples of two, which spares the launch that adds partial weight gradients; else as
-// many as fill the chip (8 x 512 x 32, forward + backward: 20 us, by one team 36)
+// teams of a group in the backward: one walks up to four samples (4 x 128 x 32, forward + backward: 22 us on the device against 18 by a
+// team a sample, but the launch that adds partial weight gradients is spared, 7 us of a call by itself); else as many as fill the chip
+// (8 x 512 x 32: 20 us, by one team 36)
 inline int gn_teams(long N, long S, int G, int q) {
-  if (N <= 2) return 1;
+  if (N <= 4) return 1;
   long k = (gn_by_wave(N, S, G, q) ? 8192 : 1024) / G;
   if (k > N) k = N;
   return (int)(k < 1 ? 1 : k);

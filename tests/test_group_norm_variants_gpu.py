@@ -71,7 +71,7 @@ def test_many_channels_after_a_call_with_few(hip_lib):
 @pytest.mark.parametrize("N,S,C,groups", [(2, 1024, 32, 8), (2, 1025, 32, 8), (2, 4096, 32, 8),        # rows of a group
                                           (32, 512, 32, 8), (33, 512, 32, 8), (600, 300, 32, 8),       # row segments altogether
                                           (3, 129, 32, 8), (8, 128, 32, 8), (9, 128, 32, 8), (33, 256, 32, 8), (12, 102, 60, 6),  # waves
-                                          (1, 7, 16, 2), (2, 7, 16, 2), (3, 7, 16, 2)])                # teams of a group
+                                          (1, 7, 16, 2), (4, 7, 16, 2), (5, 7, 16, 2)])                # teams of a group
 def test_on_both_sides_of_the_borders(hip_lib, dt, N, S, C, groups):
     x, w, b, dy = _data(N, S, C, DT[dt], seed=N + S)
     _check(x, groups, w, b, dy, "leaky_relu")
