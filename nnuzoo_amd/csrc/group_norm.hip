@@ -2,14 +2,15 @@
 //   z = (x - mu[n,g]) * r[n,g] * w[c] + b[c],  y = act(z),  mu / r over the S positions and C / G channels of a group;
 //   dz = dy act'(z),  db = sum dz,  dw = sum dz xhat,  dx = r (w dz - <w dz> - xhat <w dz xhat>)  with <.> the group's mean.
 // Bound by HBM: a group does not fit on chip, so forward reads x twice and writes y, backward reads x and dy twice and writes dx.
-// 2 x 128^3 x 32 f16 (268 MB a tensor), SiLU: sums 65 us (4.1 TB/s), write pass 90 (6.0), backward sums 131 (4.1, the logistic
-// function's share shows), write pass 151 (5.3), finishing launches 5 each.
+// 2 x 128^3 x 32 f16 (268 MB a tensor), SiLU: sums 66 us (4.1 TB/s), write pass 90 (6.0), backward sums 127 (4.2, the logistic
+// function's share shows), write pass 149 (5.4), finishing launches 5 each.
 //
-// A thread owns V consecutive channels (16 bytes) and walks the rows, a workgroup owns a run of rows of one sample: every access
+// A thread owns V consecutive channels (16 bytes) and walks the rows, a workgroup has a share of the rows of one sample: every access
 // is a run of whole rows whatever the group width, and the group's members meet only after the rows are summed.  The forward's sums
-// are fp64 (whose vector rate is that of plain fp32 here), so that E[x^2] - mu^2 loses nothing that fp32 statistics could hold,
-// whatever mu / sigma is.  Partial sums go through a workspace and are added in a fixed order: results are bit-identical from run
-// to run.  No atomics.
+// are fp64 (whose vector rate is that of plain fp32 here): E[x^2] - mu^2 then costs about 2^-53 (mu / sigma)^2 of the variance, less than
+// its rounding to fp32 up to mu / sigma = 2^14 and 2^-13 at 2^20, where x itself has 4 bits left for the spread.  Partial sums go
+// through a workspace and are added in a fixed order: results are bit-identical from run to run.
+// No atomics.
 #include "elem_io.hpp"
 
 namespace nnz {
@@ -578,8 +579,8 @@ constexpr long GN_TARGET = 1024;  // workgroups of a launch that sums
 constexpr long GN_TARGET_APPLY = 4096;  // of one that writes (1 024: 119 us instead of 89 for the forward at 2 x 128^3 x 32 f16)
 // Workgroups of a sample: enough to fill the chip, with at least 8 passes over the rows that their threads cover at once.  The rows
 // are dealt out in turn, so that the chip reads one moving window: runs of rows a workgroup lie a power of two apart on the usual
-// sizes, and their streams then meet in the same memory channels (stats / apply / reduce at 2 x 128^3 x 32 f16: 63 / 92 / 140 us
-// that way, 58 / 89 / 130 in turn).
+// sizes, and their streams then meet in the same memory channels (the forward's sums and write pass at 2 x 128^3 x 32 f16: 70 and 97 us
+// that way, 66 and 90 in turn; the backward's 128 and 145 us, and 126 and 149).
 inline void gn_split(GnArgs& a, int V, long target) {
   const int CV = a.C / V;
   const long R = CV >= GN_NT ? 1 : GN_NT / CV;

@@ -292,7 +292,9 @@ __device__ __forceinline__ ElemVec<T, 2> ld_pair(const T* p, bool aligned, int s
 // the chunks from the entry states that the summaries in front of them make: each workgroup joins up to SC_JOIN - 1 of them by
 // itself, scan_join_kernel more.
 constexpr int SC_TT = 16;   // tokens of a tile
-// chunks from which on a kernel of its own joins them (5 ragged prompts of 16 chunks: 42 us a call with it, 37 without)
+// chunks from which on a kernel of its own joins them.  Us a call with it / without, chunks of 64 tokens, fp32, 16 states: 4 x 768 channels,
+// 16 chunks 65 / 41, 31: 90 / 76, 40: 105 / 98, 64: 145 / 158; 8 x 1024 channels, 31 chunks (as many as they get): 213 / 162; 1 x 512, 16:
+// 27 / 25, 40: 34 / 34, 64: 37 / 46.  Only few channels would want it earlier: 2 x 96, 16: 24 / 26, 31: 25 / 33
 constexpr int SC_JOIN = 32;
 
 template <class T, int N, int CPL, int MODE>
